@@ -335,6 +335,68 @@ int mkb_silu_mul(const void* gate_up, void* out, int M, int I, void* stream);
  * Ranks exchange these 8 bytes per sequence instead of their logits.  logits are fp16 [M, width] with
  * row stride row_stride.  No counterpart in the reference, which leaves sampling to `transformers`. */
 int mkb_argmax(const void* logits, void* best, int M, int64_t width, int64_t row_stride, int64_t offset, void* stream);
+
+/*
+ * Attention over a paged cache.  Keys and values lie in pools of pages [pages, kv_heads, page, head_dim], fp16 or bf16, any
+ * strides that are whole 16-byte vectors, equal for both pools; slot p of sequence m is slot p % page of page
+ * tables[m, p / page] (int32, row stride table_stride, `columns` entries a row).  lengths[m] is the number of slots that
+ * sequence m holds when the call begins; a negative one marks a row that is not in use: it writes zeros and nothing else.
+ *
+ * mkb_paged_attention_decode: out[m, head, :] = softmax(q[m, head] . K[0..lengths[m]) * scale) V, zeros when the sequence
+ *     is empty.  q is [M, q_heads, head_dim] with strides of whole 16-byte vectors; out is contiguous.
+ * mkb_paged_rope_attention_decode: qkv[m] = [q_heads | kv_heads | kv_heads] x head_dim; the new key is rotated by
+ *     positions[m] (rotate-half pairing, angle position * theta^(-2i/head_dim)) and stored with the value at slot lengths[m];
+ *     the rotated queries (not rounded) attend to slots 0..lengths[m].  The caller advances lengths.  A slot that the
+ *     call writes belongs to one sequence only.
+ * weights (fp32 [pages, kv_heads, page], contiguous, may be null): every slot's softmax weight, summed over the query heads
+ *     that share its key-value head, is added; the slot of a new token begins at zero.
+ * head_dim 64, 128, 192 or 256; any number of query heads per key-value head.  What lies in slots behind a sequence's
+ * length is never used.  A length beyond the table, and an entry that is no page of the pool, never become an address:
+ * such slots are left out and mkb_decode_status is raised.
+ * workspace: mkb_paged_attention_workspace_bytes bytes (16-byte aligned), of no meaning before and after the call; calls
+ * that may run at the same time need one each.
+ * The reference has neither operator: it leaves attention to `transformers`.
+ */
+int64_t mkb_paged_attention_workspace_bytes(int M, int q_heads, int kv_heads, int head_dim, int page, int columns, int with_weights);
+int mkb_paged_attention_decode(const void* q, const int* lengths, const void* k_pages, const void* v_pages, const int* tables,
+                               void* out, float* weights, int M, int q_heads, int kv_heads, int head_dim, int page,
+                               int columns, int64_t pages, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                               int64_t table_stride, int64_t q_row_stride, int64_t q_head_stride, float scale, int dtype,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+int mkb_paged_rope_attention_decode(const void* qkv, const int* positions, const int* lengths, void* k_pages, void* v_pages,
+                                    const int* tables, void* out, float* weights, int M, int q_heads, int kv_heads,
+                                    int head_dim, int page, int columns, int64_t pages, int64_t page_stride,
+                                    int64_t head_stride, int64_t slot_stride, int64_t table_stride, int64_t qkv_row_stride,
+                                    float theta, float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+/*
+ * Eviction by accumulated attention weight: of n = lengths[m] slots head h keeps k = min(n, budget): the first `sinks`, the
+ * last `recent`, and of the others those with the largest weights (NaN below everything, a tie to the lower slot).
+ * kept[m, h, 0..k) (int32 [M, kv_heads, budget]) lists them in slot order, -1 behind; their keys, values and weights are copied
+ * to slots 0..k of the pages that new_tables names.  Those pages must be none that `tables` names, and each must be named
+ * once.  The caller swaps the tables, sets lengths to k and frees the old pages.  Layout and errors as above.
+ */
+int mkb_paged_evict(void* k_pages, void* v_pages, float* weights, const int* tables, const int* lengths, const int* new_tables,
+                    int* kept, int M, int kv_heads, int head_dim, int page, int columns, int new_columns, int64_t pages,
+                    int64_t page_stride, int64_t head_stride, int64_t slot_stride, int64_t table_stride,
+                    int64_t new_table_stride, int budget, int sinks, int recent, void* stream);
+/*
+ * Penalties, biases and a mask on logits [M, width] (dtype MKB_F16/BF16/F32, rows logits_stride apart) of the tokens
+ * offset .. offset + width, into out (may be logits itself).  For token v of row m, in fp32 in this order, rounded once:
+ *   v in tokens[m, 0..lengths[m]):                        x = x > 0 ? x / repetition[m] : x * repetition[m]
+ *   c times in tokens[m, prompts[m]..lengths[m]):         x -= frequency[m] * c;  x -= presence[m] when c > 0
+ *   entries e with bias_tokens[m, e] == v:                x += the sum of bias[m, e]
+ *   bit v % 32 of mask[m, v / 32] is 0:                   x = -infinity
+ * Each part is left out when its pointer is null (prompts: nothing is prompt; repetition: 1; frequency, presence: 0).
+ * tokens are int32, or int64 with long_tokens; ids outside this width (a negative one fills a row up) have no effect;
+ * lengths beyond `history` count as `history`.  best[m] (uint64, may be null): the word mkb_argmax gives for the result, with a
+ * 32-bit key for fp32; picked[m] (int64, may be null): the token of the largest result, the smallest on a tie.
+ */
+int mkb_adjust_logits(const void* logits, void* out, const void* tokens, const int* lengths, const int* prompts,
+                      const float* repetition, const float* frequency, const float* presence, const int* bias_tokens,
+                      const float* bias, const int* mask, void* best, void* picked, int M, int64_t width,
+                      int64_t logits_stride, int64_t out_stride, int64_t history, int64_t tokens_stride, int64_t biases,
+                      int64_t bias_stride, int64_t mask_words, int64_t mask_stride, int64_t offset, int long_tokens, int dtype,
+                      void* stream);
 /* positions[m] must lie in [0, capacity).  The kernels above never turn a position outside that range
  * into an address: they clamp it, leave the caches untouched and raise a device-wide status word.
  * mkb_decode_status reads and clears that word (non-zero: some launch since the last reading saw such

@@ -3,6 +3,7 @@
 // (grouped-query), SiLU(gate) * up.  fp16 storage, fp32 arithmetic.  They exist so that a decode step
 // is a short chain of launches that a CUDA graph replays; none of them is bandwidth critical.
 #include "mkb_common.cuh"
+#include "paged.cuh"
 
 namespace mkb {
 namespace {
@@ -511,23 +512,6 @@ __global__ void silu_mul_kernel(const __half* __restrict__ gate_up, __half* __re
   *reinterpret_cast<__half2*>(out + m * I + i) = __floats2half2_rn(act.x * u.x, act.y * u.y);
 }
 
-// Launch with the programmatic-stream-serialization attribute: the kernel may become resident while
-// its predecessor drains; it executes griddepcontrol.wait before it touches memory.
-template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, void* stream, Args... args) {
-  cudaLaunchConfig_t config{};
-  config.gridDim = grid;
-  config.blockDim = block;
-  config.dynamicSmemBytes = smem;
-  config.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attribute;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, Params(args)...);
-}
-
 }  // namespace
 }  // namespace mkb
 
@@ -698,8 +682,12 @@ extern "C" int mkb_decode_status(int* status) {
   unsigned int value = 0, zero = 0;
   cudaError_t done = cudaMemcpyFromSymbol(&value, g_decode_status, sizeof(value));
   if (done == cudaSuccess && value != 0) done = cudaMemcpyToSymbol(g_decode_status, &zero, sizeof(zero));
+  unsigned int paged = 0;
+  if (done == cudaSuccess) done = take_paged_attention_status(&paged);
+  value |= paged;
+  if (done == cudaSuccess) done = take_paged_evict_status(&paged);
   if (done != cudaSuccess) return cuda_fail(done, "decode_status");
-  *status = int(value);
+  *status = int(value | paged);
   return MKB_OK;
 }
 

@@ -35,6 +35,24 @@ struct DeviceInfo {
 };
 const DeviceInfo& device_info();
 
+// ---- launches ---------------------------------------------------------------------------------
+// Launch with the programmatic-stream-serialization attribute: the kernel may become resident while
+// its predecessor drains; it executes griddepcontrol.wait before it touches memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, void* stream, Args... args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem;
+  config.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, Params(args)...);
+}
+
 // ---- packing-word geometry -------------------------------------------------------------------
 // One word is the fewest whole bytes holding a whole number of codes.
 __host__ __device__ inline int gcd8(int bits) {

@@ -565,6 +565,201 @@ def tokens_of_keys(keys: Tensor) -> Tensor:
     return 0xFFFFFFFF - (keys & 0xFFFFFFFF)
 
 
+# ---- operators over a paged cache, and on the logits ----
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace_bytes(index: int, *shape: int) -> int:
+    """Of the device that is current, ``index``."""
+    return _native.library().mkb_paged_attention_workspace_bytes(*shape)
+
+
+def _check_pages(what: str, device: torch.device, k_pages: Tensor, v_pages: Tensor, weights: Tensor | None,
+                 *tables: Tensor) -> tuple[int, int, int, int, tuple[int, ...]]:
+    """The pool's ``(pages, kv_heads, page, head_dim)`` and the strides of its first three axes."""
+    shape, strides = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != strides or v_pages.dtype != k_pages.dtype:
+        raise ValueError(f"{what}: pages of keys and values must share one [pages, kv_heads, page, head_dim] layout and dtype")
+    if strides[3] != 1:
+        raise ValueError(f"{what}: the head dimension of the pages must be contiguous")
+    for table in tables:
+        if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1 or table.device != device:
+            raise ValueError(f"{what}: page tables are int32 [rows, columns] with contiguous rows on the device of the pages")
+    if weights is not None and (weights.dtype != torch.float32 or weights.shape != shape[:3] or not weights.is_contiguous()
+                                or weights.device != device):
+        raise ValueError(f"{what}: weights are a contiguous fp32 [pages, kv_heads, page] tensor on the device of the pages")
+    if k_pages.device != device or v_pages.device != device:
+        raise ValueError("all tensors of one call must live on one device")
+    return (*shape, strides[:3])
+
+
+def _check_rows(what: str, device: torch.device, rows: int, **vectors: Tensor) -> None:
+    for name, vector in vectors.items():
+        if vector.dtype != torch.int32 or vector.shape != (rows,) or not vector.is_contiguous() or vector.device != device:
+            raise ValueError(f"{what}: {name} must be a contiguous int32 vector of {rows} rows on the device of the pages")
+
+
+def paged_attention_decode(q: Tensor, lengths: Tensor, k_pages: Tensor, v_pages: Tensor, tables: Tensor, out: Tensor, *,
+                           scale: float | None = None, weights: Tensor | None = None) -> None:
+    """Attention of one query token per sequence (``q`` [rows, q_heads, head_dim]) to the ``lengths`` slots of its paged cache
+    (pools ``[pages, kv_heads, page, head_dim]``, page numbers ``tables`` int32 [rows, columns]) into ``out``.  An empty sequence
+    and a row that is not in use (a negative length) give zeros.  ``weights`` (fp32 [pages, kv_heads, page]) adds up every
+    slot's softmax weight over the query heads of its group."""
+    what = "paged_attention_decode"
+    if not q.is_cuda:
+        raise ValueError("mlkit_b200 kernels require CUDA tensors")
+    device, index = q.device, q.get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return paged_attention_decode(q, lengths, k_pages, v_pages, tables, out, scale=scale, weights=weights)
+    pages, kv_heads, page, head_dim, strides = _check_pages(what, device, k_pages, v_pages, weights, tables)
+    if q.dim() != 3 or q.shape[2] != head_dim or q.stride(2) != 1 or q.dtype != k_pages.dtype:
+        raise ValueError(f"{what}: queries are [rows, q_heads, {head_dim}] in the dtype of the pages with contiguous heads")
+    rows, q_heads = q.shape[:2]
+    if out.shape != q.shape and out.shape != (rows, q_heads * head_dim):
+        raise ValueError(f"{what}: the output is [rows, q_heads, head_dim]")
+    if out.dtype != q.dtype or not out.is_contiguous() or out.device != device or tables.shape[0] != rows:
+        raise ValueError(f"{what}: a contiguous output in the dtype of the queries and a row of tables for each row of queries")
+    _check_rows(what, device, rows, lengths=lengths)
+    need = _attention_workspace_bytes(index, rows, q_heads, kv_heads, head_dim, page, tables.shape[1], int(weights is not None))
+    workspace = q.new_empty(need, dtype=torch.uint8)
+    status = _native.library().mkb_paged_attention_decode(
+        q.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), out.data_ptr(),
+        _pointer(weights), rows, q_heads, kv_heads, head_dim, page, tables.shape[1], pages, *strides, tables.stride(0),
+        q.stride(0), q.stride(1), head_dim ** -0.5 if scale is None else scale, _tag(q.dtype, "cache"), workspace.data_ptr(), need,
+        torch.cuda.current_stream().cuda_stream)
+    if status:
+        _native.check(status, what)
+
+
+def paged_rope_attention_decode(qkv: Tensor, positions: Tensor, lengths: Tensor, k_pages: Tensor, v_pages: Tensor, tables: Tensor,
+                                out: Tensor, *, q_heads: int, kv_heads: int, head_dim: int, theta: float,
+                                scale: float | None = None, weights: Tensor | None = None) -> None:
+    """One decode step of attention over a paged cache: the new key of each row of ``qkv`` is rotated by ``positions`` and
+    stored with its value in slot ``lengths`` of the sequence, and the rotated queries attend to slots ``0..lengths``.  ``qkv`` is
+    left unrotated, ``lengths`` as they are; a row with a negative length is not in use (zeros, nothing stored).  Positions
+    and lengths differ where slots were evicted.  ``weights`` as in ``paged_attention_decode``; a new slot begins at zero."""
+    what = "paged_rope_attention_decode"
+    if not qkv.is_cuda:
+        raise ValueError("mlkit_b200 kernels require CUDA tensors")
+    device, index = qkv.device, qkv.get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return paged_rope_attention_decode(qkv, positions, lengths, k_pages, v_pages, tables, out, q_heads=q_heads,
+                                               kv_heads=kv_heads, head_dim=head_dim, theta=theta, scale=scale, weights=weights)
+    pages, heads, page, width, strides = _check_pages(what, device, k_pages, v_pages, weights, tables)
+    if heads != kv_heads or width != head_dim:
+        raise ValueError(f"{what}: pages of {heads} heads of {width}, asked for {kv_heads} of {head_dim}")
+    if qkv.dim() != 2 or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim or qkv.stride(1) != 1 or qkv.dtype != k_pages.dtype:
+        raise ValueError(f"{what}: q | k | v is [rows, {(q_heads + 2 * kv_heads) * head_dim}] in the dtype of the pages")
+    rows = qkv.shape[0]
+    if out.shape != (rows, q_heads * head_dim) and out.shape != (rows, q_heads, head_dim):
+        raise ValueError(f"{what}: the output is [rows, q_heads, head_dim]")
+    if out.dtype != qkv.dtype or not out.is_contiguous() or out.device != device or tables.shape[0] != rows:
+        raise ValueError(f"{what}: a contiguous output in the dtype of the queries and a row of tables for each row of queries")
+    _check_rows(what, device, rows, positions=positions, lengths=lengths)
+    need = _attention_workspace_bytes(index, rows, q_heads, kv_heads, head_dim, page, tables.shape[1], int(weights is not None))
+    workspace = qkv.new_empty(need, dtype=torch.uint8)
+    status = _native.library().mkb_paged_rope_attention_decode(
+        qkv.data_ptr(), positions.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(),
+        out.data_ptr(), _pointer(weights), rows, q_heads, kv_heads, head_dim, page, tables.shape[1], pages, *strides,
+        tables.stride(0), qkv.stride(0), theta, head_dim ** -0.5 if scale is None else scale, _tag(qkv.dtype, "cache"),
+        workspace.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    if status:
+        _native.check(status, what)
+
+
+def evict_pages(k_pages: Tensor, v_pages: Tensor, weights: Tensor, tables: Tensor, lengths: Tensor, new_tables: Tensor, *,
+                budget: int, sinks: int = 0, recent: int = 0) -> Tensor:
+    """Keep ``min(length, budget)`` slots of every sequence and head: the first ``sinks``, the last ``recent`` and the
+    heaviest of the others by ``weights`` (a tie to the lower slot).  They are copied, in slot order, to the pages that
+    ``new_tables`` names; these must be named once and be none of ``tables``.  Returns the kept slots, int32 [rows, kv_heads,
+    budget], -1 behind the last.  The caller swaps the tables, sets the lengths and frees the old pages."""
+    what = "evict_pages"
+    if not k_pages.is_cuda:
+        raise ValueError("mlkit_b200 kernels require CUDA tensors")
+    device, index = k_pages.device, k_pages.get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return evict_pages(k_pages, v_pages, weights, tables, lengths, new_tables, budget=budget, sinks=sinks, recent=recent)
+    pages, kv_heads, page, head_dim, strides = _check_pages(what, device, k_pages, v_pages, weights, tables, new_tables)
+    if k_pages.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: cache dtype {k_pages.dtype} is not supported (fp16, bf16)")
+    rows = tables.shape[0]
+    if new_tables.shape[0] != rows:
+        raise ValueError(f"{what}: a row of new tables for each row of tables")
+    _check_rows(what, device, rows, lengths=lengths)
+    kept = torch.empty((rows, kv_heads, max(budget, 0)), dtype=torch.int32, device=device)
+    status = _native.library().mkb_paged_evict(
+        k_pages.data_ptr(), v_pages.data_ptr(), weights.data_ptr(), tables.data_ptr(), lengths.data_ptr(), new_tables.data_ptr(),
+        kept.data_ptr(), rows, kv_heads, head_dim, page, tables.shape[1], new_tables.shape[1], pages, *strides, tables.stride(0),
+        new_tables.stride(0), budget, sinks, recent, torch.cuda.current_stream().cuda_stream)
+    if status:
+        _native.check(status, what)
+    return kept
+
+
+def adjust_logits(logits: Tensor, *, tokens: Tensor | None = None, lengths: Tensor | None = None, prompts: Tensor | None = None,
+                  repetition: Tensor | None = None, frequency: Tensor | None = None, presence: Tensor | None = None,
+                  bias_tokens: Tensor | None = None, bias: Tensor | None = None, mask: Tensor | None = None, offset: int = 0,
+                  best: Tensor | None = None, picked: Tensor | None = None, out: Tensor | None = None) -> Tensor:
+    """Penalties for the tokens of a history, sparse biases and a grammar's bit mask on ``logits`` [rows, width] of the tokens
+    ``offset..offset + width``; in place unless ``out`` is given.  For token v, in fp32 and in this order:
+
+    * v in ``tokens[m, :lengths[m]]``: divided by ``repetition[m]`` when positive, multiplied otherwise;
+    * c times in ``tokens[m, prompts[m]:lengths[m]]``: less ``frequency[m] * c``, and less ``presence[m]`` when c > 0;
+    * plus the ``bias`` of every entry of ``bias_tokens`` [rows, entries] that is v;
+    * -inf where bit v % 32 of ``mask[m, v // 32]`` is 0.
+
+    Ids outside ``offset..offset + width`` (-1 fills a row up) have no effect.  ``best`` (int64 [rows]) receives the words of
+    ``argmax_keys`` for the result, ``picked`` (int64 [rows]) its greedy tokens."""
+    what = "adjust_logits"
+    if not logits.is_cuda:
+        raise ValueError("mlkit_b200 kernels require CUDA tensors")
+    device, index = logits.device, logits.get_device()
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return adjust_logits(logits, tokens=tokens, lengths=lengths, prompts=prompts, repetition=repetition, frequency=frequency,
+                                 presence=presence, bias_tokens=bias_tokens, bias=bias, mask=mask, offset=offset, best=best,
+                                 picked=picked, out=out)
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError(f"{what}: logits are [rows, width] with contiguous rows")
+    rows, width = logits.shape
+    if out is None:
+        out = logits
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.stride(1) != 1 or out.device != device:
+        raise ValueError(f"{what}: the output matches the logits in shape, dtype and device, with contiguous rows")
+    if (tokens is None) != (lengths is None):
+        raise ValueError(f"{what}: a history needs its lengths")
+    if tokens is None and not (prompts is None and repetition is None and frequency is None and presence is None):
+        raise ValueError(f"{what}: penalties need a history of tokens")
+    if (bias_tokens is None) != (bias is None) or (bias is not None and bias.shape != bias_tokens.shape):
+        raise ValueError(f"{what}: biases need a token for every value")
+    for name, table, dtypes in (("tokens", tokens, (torch.int32, torch.int64)), ("bias_tokens", bias_tokens, (torch.int32,)),
+                                ("bias", bias, (torch.float32,)), ("mask", mask, (torch.int32,))):
+        if table is not None and (table.dim() != 2 or table.shape[0] != rows or table.dtype not in dtypes or table.device != device
+                                  or (table.stride(1) != 1 and table.shape[1] > 1)):
+            raise ValueError(f"{what}: {name} must be [rows, entries] of {dtypes[0]} with contiguous rows on the device of the logits")
+    for name, vector, dtype in (("lengths", lengths, torch.int32), ("prompts", prompts, torch.int32),
+                                ("repetition", repetition, torch.float32), ("frequency", frequency, torch.float32),
+                                ("presence", presence, torch.float32), ("best", best, torch.int64), ("picked", picked, torch.int64)):
+        if vector is not None and (vector.dtype != dtype or vector.shape != (rows,) or not vector.is_contiguous()
+                                   or vector.device != device):
+            raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector of {rows} rows on the device of the logits")
+    if bias is not None and bias.stride(0) != bias_tokens.stride(0):
+        raise ValueError(f"{what}: biases and their tokens must share a layout")
+    status = _native.library().mkb_adjust_logits(
+        logits.data_ptr(), out.data_ptr(), _pointer(tokens), _pointer(lengths), _pointer(prompts), _pointer(repetition),
+        _pointer(frequency), _pointer(presence), _pointer(bias_tokens), _pointer(bias), _pointer(mask), _pointer(best),
+        _pointer(picked), rows, width, logits.stride(0), out.stride(0), 0 if tokens is None else tokens.shape[1],
+        0 if tokens is None else tokens.stride(0), 0 if bias is None else bias.shape[1], 0 if bias is None else bias.stride(0),
+        0 if mask is None else mask.shape[1], 0 if mask is None else mask.stride(0), offset,
+        int(tokens is not None and tokens.dtype == torch.int64), _tag(logits.dtype, "logit"),
+        torch.cuda.current_stream().cuda_stream)
+    if status:
+        _native.check(status, what)
+    return out
+
+
 def decode_status() -> int:
     """Non-zero when a decode operator since the last call saw a cache position outside ``[0, capacity)``
     (it clamped the position and skipped the append; that step's results are not valid).  Synchronises."""
