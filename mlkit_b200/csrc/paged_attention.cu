@@ -1,6 +1,26 @@
 // Attention of one new token per sequence over a paged key-value cache.
 //   s[h, p] = scale * q[h] . k[p],   w[h, p] = exp(s[h, p] - max) / sum,   out[h] = sum_p w[h, p] v[p]
 // with the query heads h of a group sharing one key-value head; optionally acc[p] += sum over the group of w[h, p].
+//
+// What bounds it: reading the cache once, 4 * head_dim bytes a slot and key-value head for 4 * head_dim * group flops.  So:
+// * Work is cut into tiles of 16 slots of one (sequence, key-value head); the tiles of all sequences in a row are dealt out
+//   in equal runs to as many CTAs as the GPU holds, whatever the lengths.  A (sequence, head) that crosses from one CTA to
+//   the next leaves partial (max, sum, output) triples, which a second launch joins in the order of the CTAs: the
+//   workspace has two slots per CTA, independent of lengths, and there are no atomics and no state between calls.
+// * A warp copies its own tiles into a ring of its own with cp.async, several tiles ahead, across the borders of
+//   sequences.  A lane copies just those 16-byte pieces that it will itself feed to the tensor core, so that nothing in the
+//   loop waits for another lane's copy: pieces of 8 dimensions of slots g and g + 8 for the keys (g = lane / 4), of slots
+//   2t, 2t + 1, 2t + 8, 2t + 9 for the values (t = lane % 4).  Which dimension stands at which place of the products'
+//   reduction or of their rows is free as long as the queries and the outputs agree.
+// * Slots are the 16 rows of the tensor core's tile and the group's query heads its 8 columns: S^T = K Q^T, O^T = V^T P^T, so
+//   eight heads leave nothing unused and the running maximum of a column is three shuffles.  P^T turns from the accumulator's
+//   layout to the operand's with movmatrix.  More than eight heads of a group are several tiles of heads, which read the
+//   cache again (from L2, mostly).
+// * Rounding: products of 16-bit values are exact, all sums are fp32.  A softmax weight is held in two 16-bit parts (its
+//   rounding and the rest), scaled by 2^14 so that weights down to 2^-38 of the largest stay within fp16's range, and so is a
+//   rotated query: the output is rounded once, the accumulated weights are those of fp32.
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace mkb {
@@ -8,179 +28,682 @@ namespace {
 
 __device__ unsigned int g_paged_attention_status = 0;
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int offset = 16; offset; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
-  return v;
-}
+constexpr int kTile = 16;       // slots of a tile
+constexpr int kHeads = 8;       // query heads of a tile
+constexpr float kShift = 14.f;  // weights are held times 2^14
 
 struct AttentionArguments {
   PagedLayout layout;
   const void* q;
-  const int* positions;
+  const int* positions;     // with a rotation
   const int* lengths;
-  void* k_pages;
-  void* v_pages;
+  uint4* k_pages;
+  uint4* v_pages;
   void* out;
   float* weights;
   int64_t q_row, q_head;    // strides in elements
-  int q_heads, kv_heads, rope;
-  float theta, scale;
+  int rows, q_heads, kv_heads, group, head_tiles, ctas;
+  float theta, scale_log2;
+  // workspace
+  float* partial;           // [ctas][2][kHeads][head_dim]: of the item a CTA's run begins within, and of the one it ends within
+  float2* partial_norm;     // [ctas][2][kHeads]: maximum (in powers of two), sum
+  int64_t* border;          // [ctas]: the item that a CTA's run begins within, -1 when it begins with an item or is empty
+  float* norm;              // [rows][q_heads]: log2 of the softmax's sum, with weights
+  float* scores;            // [tiles][min(group, 8)][kTile], with weights
 };
 
-// cos and sin of position * theta^(-i / half): the angle in 64 bits, since a far position times a frequency rounded to 32
-// bits is off by hundredths of a turn, then reduced to a turn.
-__device__ __forceinline__ void rotation(int position, int i, int half, float theta, float& cosine, float& sine) {
-  const double turns = double(position) * exp2(-log2(double(theta)) * double(i) / double(half)) * 0.15915494309189533577;
-  sincospif(2.f * float(turns - rint(turns)), &sine, &cosine);
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+template <typename T> struct Types;
+template <> struct Types<__half> {
+  static __device__ __forceinline__ float2 widen(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+  static __device__ __forceinline__ uint32_t narrow(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+template <> struct Types<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 widen(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint32_t narrow(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+// Two floats as a pair of 16-bit values and a pair of what their rounding left out.
+template <typename T>
+__device__ __forceinline__ void split(float lo, float hi, uint32_t& pair, uint32_t& rest) {
+  pair = Types<T>::narrow(lo, hi);
+  const float2 held = Types<T>::widen(pair);
+  rest = Types<T>::narrow(lo - held.x, hi - held.y);
 }
 
-template <typename T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ uint32_t turn_matrix(uint32_t v) {   // an 8 x 8 matrix of 16-bit values across a warp, transposed
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 
-// One CTA per (key-value head, sequence); a warp takes slots, its lanes the dimensions.
-constexpr int kSimpleWarps = 8;
+// What of a sequence lies in the cache, and how many tiles it has with the token that this call adds.
+struct Extent {
+  int held, tiles, added;
+};
+template <bool Rope>
+__device__ __forceinline__ Extent extent_of(const AttentionArguments& a, int m, bool& beyond) {
+  const int n = __ldg(a.lengths + m), capacity = a.layout.capacity();
+  if (n < 0) return {0, 0, 0};
+  const int added = Rope && n < capacity;
+  if (n > capacity - Rope) beyond = true;
+  const int held = min(n, capacity);
+  return {held, (held + added + kTile - 1) / kTile, added};
+}
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kSimpleWarps * 32) paged_attention_simple_kernel(AttentionArguments a) {
+// The tiles of all sequences, (sequence, head tile, tile) in order, dealt out in equal runs.  `per_row`: head tiles of a
+// sequence; `least`: tiles that a CTA should have.  Returns the CTA's run and the (sequence, head tile, tile) it begins at.
+struct Run {
+  int64_t begin, end, total;
+  int row, head, tile;
+};
+template <bool Rope, int Threads>
+__device__ __forceinline__ Run find_run(const AttentionArguments& a, int per_row, int least, int cta, int ctas) {
+  __shared__ int64_t warp_s[Threads / 32 + 1];
+  __shared__ int found_s[3];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int each = (a.rows + Threads - 1) / Threads;
+  const int first = min(int(threadIdx.x) * each, a.rows), last = min(first + each, a.rows);
+  bool beyond = false;
+  int64_t own = 0;
+  for (int m = first; m < last; ++m) own += extent_of<Rope>(a, m, beyond).tiles;
+  if (beyond && cta == 0) atomicOr(&g_paged_attention_status, 1u);
+  int64_t before = own;
+#pragma unroll
+  for (int step = 1; step < 32; step <<= 1) {
+    const int64_t other = __shfl_up_sync(0xffffffffu, before, step);
+    if (lane >= step) before += other;
+  }
+  if (lane == 31) warp_s[warp] = before;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < Threads / 32; ++w) {
+    if (w < warp) before += warp_s[w];
+    total += warp_s[w];
+  }
+  before -= own;
+  Run run;
+  run.total = total * per_row;
+  const int64_t active = min(int64_t(ctas), max(int64_t(1), (run.total + least - 1) / least));
+  run.begin = cta < active ? run.total * cta / active : run.total;
+  run.end = cta < active ? run.total * (cta + 1) / active : run.total;
+  if (run.begin < run.end && before * per_row <= run.begin && run.begin < (before + own) * per_row) {
+    int64_t rest = run.begin - before * per_row;
+    for (int m = first; m < last; ++m) {
+      const int tiles = extent_of<Rope>(a, m, beyond).tiles;
+      if (rest < int64_t(tiles) * per_row) {
+        found_s[0] = m;
+        found_s[1] = int(rest / tiles);
+        found_s[2] = int(rest % tiles);
+        break;
+      }
+      rest -= int64_t(tiles) * per_row;
+    }
+  }
+  __syncthreads();
+  run.row = found_s[0]; run.head = found_s[1]; run.tile = found_s[2];
+  return run;
+}
+
+// A place in the order of the tiles.
+template <bool Rope>
+struct Cursor {
+  int row, head, tile;
+  Extent extent;
+  __device__ __forceinline__ void start(const AttentionArguments& a, const Run& run) {
+    bool beyond;
+    row = run.row; head = run.head; tile = run.tile;
+    extent = extent_of<Rope>(a, row, beyond);
+  }
+  // `steps` tiles on; the caller keeps it within the run.
+  __device__ __forceinline__ void advance(const AttentionArguments& a, int per_row, int steps) {
+    tile += steps;
+    while (tile >= extent.tiles) {
+      tile -= extent.tiles;
+      if (++head == per_row) {
+        head = 0;
+        bool beyond;
+        do extent = extent_of<Rope>(a, ++row, beyond); while (extent.tiles == 0);
+      }
+    }
+  }
+};
+
+template <int D> struct Shape {
+  static constexpr int kWarps = 4;
+  static constexpr int kStages = D <= 64 ? 6 : 3;
+  static constexpr int kCtas = D <= 128 ? 2 : 1;                 // per SM
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kOps = D / 16;                            // 16-byte pieces a lane copies of the keys, and of the values
+  static constexpr int kStageBytes = 2 * kOps * 32 * 16;
+  static constexpr int kRowFloats = D + 4;                       // of the outputs where the warps meet
+  static constexpr int kRing = 0;
+  static constexpr int kValid = kRing + kWarps * kStages * kStageBytes;     // [warp][stage][lane]: which of a lane's rows count
+  static constexpr int kNorm = kValid + kWarps * kStages * 32 * 4;          // [warp][head] float2
+  static constexpr int kMeet = kNorm + kWarps * kHeads * 8;                 // [warp]: the stage that holds its outputs
+  static constexpr int kTurns = kMeet + kWarps * 4;                         // [D / 2] double: turns per position
+  static constexpr int kCosine = kTurns + D / 2 * 8;                        // [D / 2][2] float
+  static constexpr int kBytes = kCosine + D / 2 * 8;
+  static_assert(kBytes <= (kCtas == 2 ? 115712 : 232448), "shared memory");
+  static_assert(kHeads * kRowFloats * 4 <= kStageBytes, "a warp's outputs fit a stage");
+};
+
+template <typename T, int D, bool Rope>
+__global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_attention_kernel(AttentionArguments a) {
+  using S = Shape<D>;
+  using Y = Types<T>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, cta = blockIdx.x;
+  const int per_row = a.kv_heads * a.head_tiles;
+  double* turns_s = reinterpret_cast<double*>(smem + S::kTurns);
+  float2* cosine_s = reinterpret_cast<float2*>(smem + S::kCosine);
+  if (Rope)   // the angle in 64 bits: a far position times a frequency rounded to 32 bits is off by hundredths of a turn
+    for (int i = threadIdx.x; i < D / 2; i += S::kThreads)
+      turns_s[i] = exp2(-log2(double(a.theta)) * double(i) / double(D / 2)) * 0.15915494309189533577;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // rows with nothing to attend to
+  for (int m = cta; m < a.rows; m += gridDim.x) {
+    bool beyond;
+    if (extent_of<Rope>(a, m, beyond).tiles == 0) {
+      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + int64_t(m) * a.q_heads * D);
+      for (int i = threadIdx.x; i < a.q_heads * D / 8; i += S::kThreads) out[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  const Run run = find_run<Rope, S::kThreads>(a, per_row, S::kWarps, cta, gridDim.x);
+  if (threadIdx.x == 0)
+    a.border[cta] = run.begin < run.end && run.tile > 0 ? (int64_t(run.row) * per_row + run.head) : -1;
+  if (run.begin >= run.end) return;
+
+  uint8_t* ring = smem + S::kRing + warp * S::kStages * S::kStageBytes + lane * 16;
+  uint32_t* valid_s = reinterpret_cast<uint32_t*>(smem + S::kValid) + warp * S::kStages * 32 + lane;
+  const int own = int(min(run.end - run.begin, int64_t(1) << 30));
+  const int mine = own > warp ? (own - warp + S::kWarps - 1) / S::kWarps : 0;   // tiles of this warp
+
+  // ---- copies: the page of a tile is looked up one tile before its copies are issued
+  Cursor<Rope> ahead;
+  ahead.start(a, run);
+  if (mine > 0) ahead.advance(a, per_row, warp);
+  uint32_t page_id = 0, inner = 0;
+  bool inside = false;
+  auto look_up = [&]() {     // of lane % 16, the slot of the tile at `ahead`
+    const uint32_t slot = uint32_t(ahead.tile) * kTile + (lane & 15);
+    inside = slot < uint32_t(ahead.extent.held);
+    if (inside) {
+      const uint32_t column = a.layout.page.quotient(slot);
+      page_id = uint32_t(__ldg(a.layout.tables + int64_t(ahead.row) * a.layout.table_stride + column));
+      inner = uint32_t(ahead.head / a.head_tiles) * a.layout.head_stride + (slot - column * a.layout.page.divisor) * a.layout.slot_stride;
+    }
+  };
+  int issued = 0;
+  auto issue = [&]() {
+    if (issued < mine) {
+      uint32_t offset = kNoSlot;
+      if (inside) {
+        if (page_id < a.layout.pages) offset = page_id * a.layout.page_stride + inner;
+        else atomicOr(&g_paged_attention_status, 1u);
+      }
+      const int stage = issued % S::kStages;
+      const uint32_t to = shared_address(ring + stage * S::kStageBytes);
+      const uint32_t rows[6] = {__shfl_sync(0xffffffffu, offset, g),         __shfl_sync(0xffffffffu, offset, g + 8),
+                                __shfl_sync(0xffffffffu, offset, 2 * t),     __shfl_sync(0xffffffffu, offset, 2 * t + 1),
+                                __shfl_sync(0xffffffffu, offset, 2 * t + 8), __shfl_sync(0xffffffffu, offset, 2 * t + 9)};
+      valid_s[stage * 32] = uint32_t(rows[0] != kNoSlot) | uint32_t(rows[1] != kNoSlot) << 1;
+      // a slot that does not count is filled with zeros: whatever lies there, a NaN too, stays out of the products
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t size = rows[r] != kNoSlot ? 16u : 0u;
+        const uint4* from = a.k_pages + (size ? int64_t(rows[r]) + t : 0);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (2 * j + r) * 512), "l"(from + (size ? 4 * j : 0)), "r"(size) : "memory");
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint32_t size = rows[2 + r] != kNoSlot ? 16u : 0u;
+        const uint4* from = a.v_pages + (size ? int64_t(rows[2 + r]) + g : 0);
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (S::kOps + 4 * j + r) * 512), "l"(from + (size ? 8 * j : 0)), "r"(size) : "memory");
+      }
+      if (++issued < mine) {
+        ahead.advance(a, per_row, S::kWarps);
+        look_up();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (mine > 0) look_up();
+#pragma unroll
+  for (int i = 0; i < S::kStages - 1; ++i) issue();
+
+  // ---- the run, item by item
+  Cursor<Rope> at;
+  at.start(a, run);
+  int turned = -1, taken = 0;
+  for (int64_t done = run.begin; done < run.end;) {
+    const int count = int(min(int64_t(at.extent.tiles - at.tile), run.end - done));
+    const int kv = at.head / a.head_tiles, head0 = kv * a.group + (at.head - kv * a.head_tiles) * kHeads;
+    const int heads = min(kHeads, a.group - (at.head - kv * a.head_tiles) * kHeads);
+    const T* source = static_cast<const T*>(a.q) + int64_t(at.row) * a.q_row;
+    if (Rope && turned != at.row) {
+      turned = at.row;
+      const double position = double(__ldg(a.positions + at.row));
+      __syncthreads();
+      for (int i = threadIdx.x; i < D / 2; i += S::kThreads) {
+        const double turns = position * turns_s[i];
+        float sine, cosine;
+        sincospif(2.f * float(turns - rint(turns)), &sine, &cosine);
+        cosine_s[i] = make_float2(cosine, sine);
+      }
+      __syncthreads();
+    }
+    // rotates pieces of 8 dimensions d.. and d + D/2.. of a row
+    auto rotate = [&](const uint4& low, const uint4& high, int d, float (&x)[8], float (&y)[8]) {
+      const uint32_t l[4] = {low.x, low.y, low.z, low.w}, h[4] = {high.x, high.y, high.z, high.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 p = Y::widen(l[i]), q = Y::widen(h[i]), c0 = cosine_s[d + 2 * i], c1 = cosine_s[d + 2 * i + 1];
+        x[2 * i] = p.x * c0.x - q.x * c0.y;
+        x[2 * i + 1] = p.y * c1.x - q.y * c1.y;
+        y[2 * i] = q.x * c0.x + p.x * c0.y;
+        y[2 * i + 1] = q.y * c1.x + p.y * c1.y;
+      }
+    };
+    // queries: head g, dimensions 32j + 8t ..
+    uint32_t query[D / 32][4], rest[Rope ? D / 32 : 1][4];
+    {
+      const uint4* q = reinterpret_cast<const uint4*>(source + int64_t(head0 + g) * a.q_head) + t;
+      uint4 raw[D / 32];
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) raw[j] = g < heads ? __ldg(q + 4 * j) : make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (Rope) {
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+          float x[8], y[8];
+          rotate(raw[j], raw[j + D / 64], 32 * j + 8 * t, x, y);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            split<T>(x[2 * i], x[2 * i + 1], query[j][i], rest[j][i]);
+            split<T>(y[2 * i], y[2 * i + 1], query[j + D / 64][i], rest[j + D / 64][i]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          query[j][0] = raw[j].x; query[j][1] = raw[j].y; query[j][2] = raw[j].z; query[j][3] = raw[j].w;
+        }
+      }
+    }
+    float out[D / 16][4];   // [64j.. : 4j + i]: dimensions 64j + 8g + 2i (0, 1) and + 1 (2, 3) of heads 2t and 2t + 1
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) out[i][0] = out[i][1] = out[i][2] = out[i][3] = 0.f;
+    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+
+    const int skip = int((done - run.begin) % S::kWarps);
+    for (int i = warp >= skip ? warp - skip : warp - skip + S::kWarps; i < count; i += S::kWarps) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+      issue();     // into the stage of the tile before, whose pieces the products have taken
+      const int stage = taken++ % S::kStages;
+      uint8_t* from = ring + stage * S::kStageBytes;
+      uint32_t valid = valid_s[stage * 32];
+      const int tile = at.tile + i;
+      if (Rope && at.extent.added && tile == at.extent.held / kTile) {
+        // the token that this call adds: the lanes that hold pieces of its row put them into their rings and the cache
+        const int r = at.extent.held % kTile;
+        const uint32_t slot = a.layout.vector_of(a.layout.tables + int64_t(at.row) * a.layout.table_stride, kv, at.extent.held);
+        const bool store = slot != kNoSlot && at.head == kv * a.head_tiles;
+        if (slot == kNoSlot) {
+          atomicOr(&g_paged_attention_status, 1u);
+        } else {
+          if ((r & 7) == g) {
+            const uint4* k = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + kv) * D) + t;
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+              float x[8], y[8];
+              rotate(__ldg(k + 4 * j), __ldg(k + 4 * (j + D / 64)), 32 * j + 8 * t, x, y);
+              const uint4 low = make_uint4(Y::narrow(x[0], x[1]), Y::narrow(x[2], x[3]), Y::narrow(x[4], x[5]), Y::narrow(x[6], x[7]));
+              const uint4 high = make_uint4(Y::narrow(y[0], y[1]), Y::narrow(y[2], y[3]), Y::narrow(y[4], y[5]), Y::narrow(y[6], y[7]));
+              *reinterpret_cast<uint4*>(from + (2 * j + (r >> 3)) * 512) = low;
+              *reinterpret_cast<uint4*>(from + (2 * (j + D / 64) + (r >> 3)) * 512) = high;
+              if (store) {
+                a.k_pages[int64_t(slot) + 4 * j + t] = low;
+                a.k_pages[int64_t(slot) + 4 * (j + D / 64) + t] = high;
+              }
+            }
+            valid |= 1u << (r >> 3);
+          }
+          if (((r & 7) >> 1) == t) {
+            const uint4* v = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + a.kv_heads + kv) * D) + g;
+#pragma unroll
+            for (int j = 0; j < D / 64; ++j) {
+              const uint4 piece = __ldg(v + 8 * j);
+              *reinterpret_cast<uint4*>(from + (S::kOps + 4 * j + (r >> 3) * 2 + (r & 1)) * 512) = piece;
+              if (store) a.v_pages[int64_t(slot) + 8 * j + g] = piece;
+            }
+          }
+        }
+        __syncwarp();
+      }
+      // scores of slots g (0, 1) and g + 8 (2, 3) for heads 2t and 2t + 1
+      float score[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const uint4 x = *reinterpret_cast<const uint4*>(from + (2 * j) * 512), y = *reinterpret_cast<const uint4*>(from + (2 * j + 1) * 512);
+        Y::mma(score, x.x, y.x, x.y, y.y, query[j][0], query[j][1]);
+        Y::mma(Rope ? score : small, x.z, y.z, x.w, y.w, query[j][2], query[j][3]);
+        if constexpr (Rope) {
+          Y::mma(small, x.x, y.x, x.y, y.y, rest[j][0], rest[j][1]);
+          Y::mma(small, x.z, y.z, x.w, y.w, rest[j][2], rest[j][3]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) score[e] = valid >> (e >> 1) & 1u ? (score[e] + small[e]) * a.scale_log2 : -INFINITY;
+      if (a.weights != nullptr) {
+        float* to = a.scores + (done + i) * (int64_t(min(a.group, kHeads)) * kTile);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (2 * t + (e & 1) < heads) to[(2 * t + (e & 1)) * kTile + g + (e >> 1) * 8] = score[e];
+      }
+      float high[2] = {fmaxf(score[0], score[2]), fmaxf(score[1], score[3])};
+#pragma unroll
+      for (int step = 4; step < 32; step <<= 1) {
+        high[0] = fmaxf(high[0], __shfl_xor_sync(0xffffffffu, high[0], step));
+        high[1] = fmaxf(high[1], __shfl_xor_sync(0xffffffffu, high[1], step));
+      }
+      if (__any_sync(0xffffffffu, high[0] > top[0] || high[1] > top[1])) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float now = fmaxf(top[c], high[c]);
+          const float fade = now > -INFINITY ? exp2f(top[c] - now) : 1.f;
+          top[c] = now;
+          sum[c] *= fade;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) { out[k][c] *= fade; out[k][c + 2] *= fade; }
+        }
+      }
+      const float base[2] = {top[0] > -INFINITY ? top[0] - kShift : 0.f, top[1] > -INFINITY ? top[1] - kShift : 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        score[e] = exp2f(score[e] - base[e & 1]);
+        sum[e & 1] += score[e];
+      }
+      uint32_t p0, p1, r0, r1;
+      split<T>(score[0], score[1], p0, r0);
+      split<T>(score[2], score[3], p1, r1);
+      p0 = turn_matrix(p0); p1 = turn_matrix(p1); r0 = turn_matrix(r0); r1 = turn_matrix(r1);
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        uint4 v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const uint4*>(from + (S::kOps + 4 * j + r) * 512);
+        const uint32_t words[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                      {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t a0 = __byte_perm(words[0][k], words[1][k], 0x5410), a1 = __byte_perm(words[0][k], words[1][k], 0x7632);
+          const uint32_t a2 = __byte_perm(words[2][k], words[3][k], 0x5410), a3 = __byte_perm(words[2][k], words[3][k], 0x7632);
+          Y::mma(out[4 * j + k], a0, a1, a2, a3, p0, p1);
+          Y::mma(out[4 * j + k], a0, a1, a2, a3, r0, r1);
+        }
+      }
+    }
+
+    // ---- the warps meet, each in the stage of its ring that no copy is under way to
+#pragma unroll
+    for (int step = 4; step < 32; step <<= 1) {
+      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], step);
+      sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], step);
+    }
+    const int free_stage = (taken + S::kStages - 1) % S::kStages;
+    float* out_s = reinterpret_cast<float*>(ring - lane * 16 + free_stage * S::kStageBytes);
+    float2* norm_s = reinterpret_cast<float2*>(smem + S::kNorm);
+    int* meet_s = reinterpret_cast<int*>(smem + S::kMeet);
+    if (lane == 0) meet_s[warp] = S::kRing + (warp * S::kStages + free_stage) * S::kStageBytes;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int head = 2 * t + c;
+      if (g == 0) norm_s[warp * kHeads + head] = make_float2(top[c], sum[c]);
+      float* row = out_s + head * S::kRowFloats + 8 * g;
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        *reinterpret_cast<float4*>(row + 64 * j) = make_float4(out[4 * j][c], out[4 * j][c + 2], out[4 * j + 1][c], out[4 * j + 1][c + 2]);
+        *reinterpret_cast<float4*>(row + 64 * j + 4) = make_float4(out[4 * j + 2][c], out[4 * j + 2][c + 2], out[4 * j + 3][c], out[4 * j + 3][c + 2]);
+      }
+    }
+    __syncthreads();
+    const bool from_start = at.tile == 0, to_end = at.tile + count == at.extent.tiles;
+    for (int index = threadIdx.x; index < heads * (D / 8); index += S::kThreads) {
+      const int head = index / (D / 8), d = (index - head * (D / 8)) * 8;
+      float all = -INFINITY, total = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < S::kWarps; ++w) all = fmaxf(all, norm_s[w * kHeads + head].x);
+#pragma unroll
+      for (int w = 0; w < S::kWarps; ++w) {
+        const float2 norm = norm_s[w * kHeads + head];
+        if (norm.y == 0.f) continue;            // no tiles, or none whose slots count
+        const float fade = exp2f(norm.x - all);
+        total += norm.y * fade;
+        const float4* row = reinterpret_cast<const float4*>(smem + meet_s[w] + (head * S::kRowFloats + d) * 4);
+        const float4 lo = row[0], hi = row[1];
+        x[0] += lo.x * fade; x[1] += lo.y * fade; x[2] += lo.z * fade; x[3] += lo.w * fade;
+        x[4] += hi.x * fade; x[5] += hi.y * fade; x[6] += hi.z * fade; x[7] += hi.w * fade;
+      }
+      if (from_start && to_end) {
+        const float inverse = total == 0.f ? 0.f : 1.f / total;
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (int64_t(at.row) * a.q_heads + head0 + head) * D + d) =
+            make_uint4(Y::narrow(x[0] * inverse, x[1] * inverse), Y::narrow(x[2] * inverse, x[3] * inverse),
+                       Y::narrow(x[4] * inverse, x[5] * inverse), Y::narrow(x[6] * inverse, x[7] * inverse));
+        if (a.weights != nullptr && d == 0) a.norm[int64_t(at.row) * a.q_heads + head0 + head] = all - kShift + log2f(total);
+      } else {
+        const int64_t slot = (int64_t(cta) * 2 + from_start) * kHeads + head;
+        float4* row = reinterpret_cast<float4*>(a.partial + slot * D + d);
+        row[0] = make_float4(x[0], x[1], x[2], x[3]);
+        row[1] = make_float4(x[4], x[5], x[6], x[7]);
+        if (d == 0) a.partial_norm[slot] = make_float2(all, total);
+      }
+    }
+    done += count;
+    if (done < run.end) {
+      at.advance(a, per_row, count);
+      __syncthreads();
+    }
+  }
+}
+
+// A block per border between two CTAs and head of a tile: the first border within an item joins all that the item left.
+constexpr int kJoinThreads = 256;
+
+template <typename T, int D, bool Rope>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(AttentionArguments a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int L = D / 32;
-  __shared__ float q_s[D], acc_s[kSimpleWarps][D], max_s[kSimpleWarps], sum_s[kSimpleWarps];
-  extern __shared__ float norm_s[];   // [group][2]
-  const int kv = blockIdx.x, m = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.q_heads / a.kv_heads, capacity = a.layout.capacity();
-  const int* table = a.layout.tables + m * a.layout.table_stride;
-  const T* source = static_cast<const T*>(a.q) + m * a.q_row;
-  int length = a.lengths[m];
-  const bool idle = length < 0;
-  if (length > capacity - a.rope) {
-    if (threadIdx.x == 0) atomicOr(&g_paged_attention_status, 1u);
-    length = capacity;
-  } else if (a.rope && !idle) {
-    const uint32_t at = a.layout.vector_of(table, kv, length);
-    if (at == kNoSlot) {
-      if (threadIdx.x == 0) atomicOr(&g_paged_attention_status, 1u);
-    } else {
-      const T* k = source + int64_t(a.q_heads + kv) * D;
-      const T* v = k + int64_t(a.kv_heads) * D;
-      for (int i = threadIdx.x; i < D / 2; i += blockDim.x) {
-        float cosine, sine;
-        rotation(a.positions[m], i, D / 2, a.theta, cosine, sine);
-        const float lo = to_float(k[i]), hi = to_float(k[i + D / 2]);
-        static_cast<T*>(a.k_pages)[int64_t(at) * 8 + i] = from_float<T>(lo * cosine - hi * sine);
-        static_cast<T*>(a.k_pages)[int64_t(at) * 8 + i + D / 2] = from_float<T>(hi * cosine + lo * sine);
+  constexpr int kLanes = D / 4, kParts = kJoinThreads / kLanes;    // threads of one partial, partials at a time
+  __shared__ float4 out_s[kParts][kLanes];
+  __shared__ float sum_s[kParts];
+  const int cta = blockIdx.x + 1, head = blockIdx.y;
+  const int64_t item = a.border[cta];
+  if (item < 0 || a.border[cta - 1] == item) return;
+  const int per_row = a.kv_heads * a.head_tiles, row = int(item / per_row), tile = int(item - int64_t(row) * per_row);
+  const int kv = tile / a.head_tiles, first = (tile - kv * a.head_tiles) * kHeads;
+  if (head >= min(kHeads, a.group - first)) return;
+  int count = 1;     // partials: the tail of the CTA before, and the heads of those that begin within the item
+  for (int i = cta; i < a.ctas; i += kJoinThreads) count += __syncthreads_count(i + threadIdx.x < a.ctas && a.border[min(i + int(threadIdx.x), a.ctas - 1)] == item);
+  auto slot_of = [&](int i) { return (i == 0 ? int64_t(cta - 1) * 2 + 1 : int64_t(cta + i - 1) * 2) * kHeads + head; };
+  float top = -INFINITY;
+  for (int i = threadIdx.x & 31; i < count; i += 32) top = fmaxf(top, a.partial_norm[slot_of(i)].x);
+#pragma unroll
+  for (int step = 16; step; step >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+  const int part = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  if (part < kParts) {
+#pragma unroll 4
+    for (int i = part; i < count; i += kParts) {
+      const float2 norm = a.partial_norm[slot_of(i)];
+      const float4 v = reinterpret_cast<const float4*>(a.partial + slot_of(i) * D)[lane];
+      const float fade = norm.x > -INFINITY ? exp2f(norm.x - top) : 0.f;
+      sum += norm.y * fade;
+      x.x += v.x * fade; x.y += v.y * fade; x.z += v.z * fade; x.w += v.w * fade;
+    }
+    out_s[part][lane] = x;
+    if (lane == 0) sum_s[part] = sum;
+  }
+  __syncthreads();
+  if (part != 0) return;
+  for (int i = 1; i < kParts; ++i) {
+    const float4 v = out_s[i][lane];
+    x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
+    sum += sum_s[i];
+  }
+  const float inverse = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t query = int64_t(row) * a.q_heads + kv * a.group + first + head;
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + query * D + lane * 4) =
+      make_uint2(Types<T>::narrow(x.x * inverse, x.y * inverse), Types<T>::narrow(x.z * inverse, x.w * inverse));
+  if (a.weights != nullptr && lane == 0) a.norm[query] = top - kShift + log2f(sum);
+}
+
+// acc[slot] += the weights of the group's heads, from the scores that the first launch left.  A half warp per tile of 16
+// slots; the heads are added in their order.
+constexpr int kWeightThreads = 256;
+
+template <bool Rope>
+__global__ void __launch_bounds__(kWeightThreads) paged_weight_kernel(AttentionArguments a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int kParts = kWeightThreads / kTile;
+  const Run run = find_run<Rope, kWeightThreads>(a, a.kv_heads, kParts, blockIdx.x, gridDim.x);
+  if (run.begin >= run.end) return;
+  const int part = threadIdx.x / kTile, lane = threadIdx.x % kTile, stored = min(a.group, kHeads);
+  if (part >= run.end - run.begin) return;
+  Cursor<Rope> at;
+  at.start(a, run);
+  int64_t before = run.begin - (int64_t(at.head) * at.extent.tiles + at.tile);      // tiles of the rows before
+  int row = at.row;
+  at.advance(a, a.kv_heads, part);
+  auto catch_up = [&]() {
+    for (; row < at.row; ++row) {
+      bool beyond;
+      before += int64_t(extent_of<Rope>(a, row, beyond).tiles) * a.kv_heads;
+    }
+  };
+  for (int64_t done = run.begin + part;;) {
+    catch_up();
+    const int slot = at.tile * kTile + lane;
+    const int* table = a.layout.tables + int64_t(at.row) * a.layout.table_stride;
+    if (slot < at.extent.held + at.extent.added) {
+      const int64_t to = a.layout.weight_of(table, a.kv_heads, at.head, slot);
+      if (to >= 0) {
+        const bool added = slot == at.extent.held;
+        float total = 0.f;
+        for (int tile = 0; tile < a.head_tiles; ++tile) {
+          // the scores lie in the order of the first launch: (row, head, head tile, tile)
+          const int64_t from = before * a.head_tiles + (int64_t(at.head) * a.head_tiles + tile) * at.extent.tiles + at.tile;
+          const int heads = min(kHeads, a.group - tile * kHeads);
+          const float* norm = a.norm + int64_t(at.row) * a.q_heads + at.head * a.group + tile * kHeads;
+          for (int h = 0; h < heads; ++h) total += exp2f(a.scores[(from * stored + h) * kTile + lane] - norm[h]);
+        }
+        a.weights[to] = added ? total : a.weights[to] + total;
       }
-      for (int i = threadIdx.x; i < D; i += blockDim.x) static_cast<T*>(a.v_pages)[int64_t(at) * 8 + i] = v[i];
-      if (a.weights != nullptr && threadIdx.x == 0) a.weights[a.layout.weight_of(table, a.kv_heads, kv, length)] = 0.f;
     }
-    ++length;
-  }
-  auto load_query = [&](int head) {
-    __syncthreads();
-    const T* q = source + int64_t(head) * a.q_head;
-    for (int i = threadIdx.x; i < D / 2; i += blockDim.x) {
-      float lo = to_float(q[i]), hi = to_float(q[i + D / 2]), cosine = 1.f, sine = 0.f;
-      if (a.rope) rotation(a.positions[m], i, D / 2, a.theta, cosine, sine);
-      q_s[i] = (lo * cosine - hi * sine) * a.scale;
-      q_s[i + D / 2] = (hi * cosine + lo * sine) * a.scale;
-    }
-    __syncthreads();
-  };
-  auto score = [&](int p, uint32_t& at) {
-    at = a.layout.vector_of(table, kv, p);
-    if (at == kNoSlot) {
-      if (lane == 0) atomicOr(&g_paged_attention_status, 1u);
-      return -INFINITY;
-    }
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < L; ++i) dot += q_s[i * 32 + lane] * to_float(static_cast<const T*>(a.k_pages)[int64_t(at) * 8 + i * 32 + lane]);
-    return warp_sum(dot);
-  };
-  for (int g = 0; g < group; ++g) {
-    const int head = kv * group + g;
-    load_query(head);
-    float top = -INFINITY, sum = 0.f, acc[L];
-#pragma unroll
-    for (int i = 0; i < L; ++i) acc[i] = 0.f;
-    for (int p = warp; p < length; p += kSimpleWarps) {
-      uint32_t at;
-      const float s = score(p, at);
-      if (at == kNoSlot) continue;
-      const float now = fmaxf(top, s), old = expf(top - now), w = expf(s - now);
-      top = now;
-      sum = sum * old + w;
-#pragma unroll
-      for (int i = 0; i < L; ++i) acc[i] = acc[i] * old + w * to_float(static_cast<const T*>(a.v_pages)[int64_t(at) * 8 + i * 32 + lane]);
-    }
-    if (lane == 0) { max_s[warp] = top; sum_s[warp] = sum; }
-#pragma unroll
-    for (int i = 0; i < L; ++i) acc_s[warp][i * 32 + lane] = acc[i];
-    __syncthreads();
-    float all = -INFINITY, total = 0.f;
-    for (int w = 0; w < kSimpleWarps; ++w) all = fmaxf(all, max_s[w]);
-    for (int w = 0; w < kSimpleWarps; ++w) total += max_s[w] > -INFINITY ? sum_s[w] * expf(max_s[w] - all) : 0.f;
-    for (int i = threadIdx.x; i < D; i += blockDim.x) {
-      float value = 0.f;
-      for (int w = 0; w < kSimpleWarps; ++w) value += max_s[w] > -INFINITY ? acc_s[w][i] * expf(max_s[w] - all) : 0.f;
-      static_cast<T*>(a.out)[(int64_t(m) * a.q_heads + head) * D + i] = from_float<T>(length > 0 && total != 0.f ? value / total : 0.f);
-    }
-    if (threadIdx.x == 0) { norm_s[2 * g] = all; norm_s[2 * g + 1] = total; }
-  }
-  if (a.weights == nullptr) return;
-  for (int g = 0; g < group; ++g) {
-    load_query(kv * group + g);
-    for (int p = warp; p < length; p += kSimpleWarps) {
-      uint32_t at;
-      const float s = score(p, at);
-      if (at != kNoSlot && lane == 0) a.weights[a.layout.weight_of(table, a.kv_heads, kv, p)] += expf(s - norm_s[2 * g]) / norm_s[2 * g + 1];
-    }
+    done += kParts;
+    if (done >= run.end) break;
+    at.advance(a, a.kv_heads, kParts);
   }
 }
 
-template <typename T, int D>
-int launch(const AttentionArguments& a, int M, void* stream) {
-  const cudaError_t launched = launch_dependent(paged_attention_simple_kernel<T, D>, dim3(a.kv_heads, M), dim3(kSimpleWarps * 32),
-                                                size_t(a.q_heads / a.kv_heads) * 8, stream, a);
+int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// CTAs of the first launch, and where the parts of its workspace begin.
+struct Workspace {
+  int ctas;
+  int64_t partial, partial_norm, border, norm, scores, bytes;
+  Workspace(int rows, int q_heads, int kv_heads, int head_dim, int page, int columns, bool weights) {
+    ctas = device_info().sm_count * (head_dim <= 128 ? 2 : 1);
+    const int group = q_heads / kv_heads, head_tiles = (group + kHeads - 1) / kHeads;
+    partial = 0;
+    partial_norm = partial + aligned(int64_t(ctas) * 2 * kHeads * head_dim * 4);
+    border = partial_norm + aligned(int64_t(ctas) * 2 * kHeads * 8);
+    norm = border + aligned(int64_t(ctas) * 8);
+    scores = norm + (weights ? aligned(int64_t(rows) * q_heads * 4) : 0);
+    const int64_t tiles = int64_t(rows) * kv_heads * head_tiles * ((int64_t(columns) * page + kTile - 1) / kTile);
+    bytes = scores + (weights ? aligned(tiles * (group < kHeads ? group : kHeads) * kTile * 4) : 0);
+  }
+};
+
+template <typename T, int D, bool Rope>
+int launch(AttentionArguments& a, void* stream) {
+  using S = Shape<D>;
+  int device = 0;
+  cudaGetDevice(&device);
+  static std::atomic<uint64_t> opted{0};
+  if (!(opted.load(std::memory_order_acquire) >> (device & 63) & 1)) {
+    const cudaError_t set = cudaFuncSetAttribute(paged_attention_kernel<T, D, Rope>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (set != cudaSuccess) return cuda_fail(set, "paged attention shared memory");
+    opted.fetch_or(uint64_t(1) << (device & 63), std::memory_order_release);
+  }
+  cudaError_t launched = launch_dependent(paged_attention_kernel<T, D, Rope>, dim3(a.ctas), dim3(S::kThreads), S::kBytes, stream, a);
+  if (launched == cudaSuccess)
+    launched = launch_dependent(paged_join_kernel<T, D, Rope>, dim3(a.ctas - 1, a.group < kHeads ? a.group : kHeads), dim3(kJoinThreads), 0, stream, a);
+  if (launched == cudaSuccess && a.weights != nullptr)
+    launched = launch_dependent(paged_weight_kernel<Rope>, dim3(a.ctas * 2), dim3(kWeightThreads), 0, stream, a);
   if (launched != cudaSuccess) return cuda_fail(launched, "paged attention launch");
   return MKB_OK;
 }
 
-int dispatch(const AttentionArguments& a, int M, int head_dim, int dtype, void* stream) {
-  if (dtype == MKB_F16) {
-    switch (head_dim) {
-      case 64: return launch<__half, 64>(a, M, stream);
-      case 128: return launch<__half, 128>(a, M, stream);
-      case 192: return launch<__half, 192>(a, M, stream);
-      default: return launch<__half, 256>(a, M, stream);
-    }
-  }
+template <typename T, bool Rope>
+int dispatch(AttentionArguments& a, int head_dim, void* stream) {
   switch (head_dim) {
-    case 64: return launch<__nv_bfloat16, 64>(a, M, stream);
-    case 128: return launch<__nv_bfloat16, 128>(a, M, stream);
-    case 192: return launch<__nv_bfloat16, 192>(a, M, stream);
-    default: return launch<__nv_bfloat16, 256>(a, M, stream);
+    case 64: return launch<T, 64, Rope>(a, stream);
+    case 128: return launch<T, 128, Rope>(a, stream);
+    case 192: return launch<T, 192, Rope>(a, stream);
+    default: return launch<T, 256, Rope>(a, stream);
   }
 }
 
-int check(const char* what, const void* q, const int* lengths, const void* out, const float* weights, int M, int q_heads,
-          int kv_heads, int head_dim, int64_t q_row, int64_t q_head, int dtype, float scale, const void* workspace,
-          int64_t workspace_bytes, int64_t need) {
-  MKB_REQUIRE(q && lengths && out, MKB_E_ARGUMENT, "%s: null pointer", what);
+// Checks what both entry points share, fills the rest of `a` and launches.
+int attend(const char* what, AttentionArguments& a, bool rope, void* out, float* weights, int M, int q_heads, int kv_heads, int head_dim,
+           int page, int columns, float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  MKB_REQUIRE(a.q && a.lengths && out && (a.positions || !rope), MKB_E_ARGUMENT, "%s: null pointer", what);
   MKB_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0, MKB_E_ARGUMENT, "%s: %d query heads for %d key-value heads", what, q_heads, kv_heads);
   MKB_REQUIRE(dtype == MKB_F16 || dtype == MKB_BF16, MKB_E_UNSUPPORTED, "%s: dtype tag %d (fp16 and bf16 supported)", what, dtype);
-  MKB_REQUIRE(M <= 65535 && kv_heads <= 65535 && q_heads <= 1 << 20, MKB_E_UNSUPPORTED, "%s: %d sequences of %d heads", what, M, q_heads);
-  MKB_REQUIRE(scale == scale && fabsf(scale) < INFINITY, MKB_E_ARGUMENT, "%s: scale is not finite", what);
-  MKB_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 && q_row % 8 == 0 && q_head % 8 == 0,
+  MKB_REQUIRE(M <= 65535 && q_heads <= 65535, MKB_E_UNSUPPORTED, "%s: %d sequences of %d heads", what, M, q_heads);
+  MKB_REQUIRE(fabsf(scale) < INFINITY, MKB_E_ARGUMENT, "%s: scale is not finite", what);
+  MKB_REQUIRE(((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 && a.q_row % 8 == 0 && a.q_head % 8 == 0,
               MKB_E_ALIGNMENT, "%s: queries and outputs lie on 16-byte vectors", what);
-  MKB_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)),
-              MKB_E_ARGUMENT, "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)need);
-  return MKB_OK;
+  const Workspace parts(M, q_heads, kv_heads, head_dim, page, columns, weights != nullptr);
+  MKB_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= parts.bytes, MKB_E_ARGUMENT,
+              "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)parts.bytes);
+  char* base = static_cast<char*>(workspace);
+  a.out = out; a.weights = weights; a.rows = M; a.q_heads = q_heads; a.kv_heads = kv_heads; a.group = q_heads / kv_heads;
+  a.head_tiles = (a.group + kHeads - 1) / kHeads; a.ctas = parts.ctas;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.partial = reinterpret_cast<float*>(base + parts.partial);
+  a.partial_norm = reinterpret_cast<float2*>(base + parts.partial_norm);
+  a.border = reinterpret_cast<int64_t*>(base + parts.border);
+  a.norm = reinterpret_cast<float*>(base + parts.norm);
+  a.scores = reinterpret_cast<float*>(base + parts.scores);
+  if (dtype == MKB_F16) return rope ? dispatch<__half, true>(a, head_dim, stream) : dispatch<__half, false>(a, head_dim, stream);
+  return rope ? dispatch<__nv_bfloat16, true>(a, head_dim, stream) : dispatch<__nv_bfloat16, false>(a, head_dim, stream);
 }
 
 }  // namespace
@@ -216,8 +739,8 @@ cudaError_t take_paged_attention_status(unsigned int* value) {
 
 extern "C" int64_t mkb_paged_attention_workspace_bytes(int M, int q_heads, int kv_heads, int head_dim, int page, int columns,
                                                        int with_weights) {
-  if (M <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || page <= 0 || columns <= 0) return 0;
-  return 0;
+  if (M <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_dim <= 0 || page <= 0 || columns <= 0) return 0;
+  return mkb::Workspace(M, q_heads, kv_heads, head_dim, page, columns, with_weights != 0).bytes;
 }
 
 extern "C" int mkb_paged_attention_decode(const void* q, const int* lengths, const void* k_pages, const void* v_pages,
@@ -231,15 +754,12 @@ extern "C" int mkb_paged_attention_decode(const void* q, const int* lengths, con
   MKB_REQUIRE(M >= 0, MKB_E_ARGUMENT, "%s: bad shape", what);
   if (M == 0) return MKB_OK;
   AttentionArguments a{};
-  int status = paged_layout(&a.layout, what, k_pages, v_pages, tables, kv_heads, head_dim, page, columns, pages, page_stride, head_stride,
-                            slot_stride, table_stride);
+  const int status = paged_layout(&a.layout, what, k_pages, v_pages, tables, kv_heads, head_dim, page, columns, pages, page_stride,
+                                  head_stride, slot_stride, table_stride);
   if (status != MKB_OK) return status;
-  status = check(what, q, lengths, out, weights, M, q_heads, kv_heads, head_dim, q_row_stride, q_head_stride, dtype, scale, workspace,
-                 workspace_bytes, mkb_paged_attention_workspace_bytes(M, q_heads, kv_heads, head_dim, page, columns, weights != nullptr));
-  if (status != MKB_OK) return status;
-  a.q = q; a.lengths = lengths; a.k_pages = const_cast<void*>(k_pages); a.v_pages = const_cast<void*>(v_pages); a.out = out;
-  a.weights = weights; a.q_row = q_row_stride; a.q_head = q_head_stride; a.q_heads = q_heads; a.kv_heads = kv_heads; a.scale = scale;
-  return dispatch(a, M, head_dim, dtype, stream);
+  a.q = q; a.lengths = lengths; a.q_row = q_row_stride; a.q_head = q_head_stride;
+  a.k_pages = static_cast<uint4*>(const_cast<void*>(k_pages)); a.v_pages = static_cast<uint4*>(const_cast<void*>(v_pages));
+  return attend(what, a, false, out, weights, M, q_heads, kv_heads, head_dim, page, columns, scale, dtype, workspace, workspace_bytes, stream);
 }
 
 extern "C" int mkb_paged_rope_attention_decode(const void* qkv, const int* positions, const int* lengths, void* k_pages, void* v_pages,
@@ -253,15 +773,11 @@ extern "C" int mkb_paged_rope_attention_decode(const void* qkv, const int* posit
   MKB_REQUIRE(M >= 0, MKB_E_ARGUMENT, "%s: bad shape", what);
   if (M == 0) return MKB_OK;
   AttentionArguments a{};
-  int status = paged_layout(&a.layout, what, k_pages, v_pages, tables, kv_heads, head_dim, page, columns, pages, page_stride, head_stride,
-                            slot_stride, table_stride);
+  const int status = paged_layout(&a.layout, what, k_pages, v_pages, tables, kv_heads, head_dim, page, columns, pages, page_stride,
+                                  head_stride, slot_stride, table_stride);
   if (status != MKB_OK) return status;
-  MKB_REQUIRE(positions, MKB_E_ARGUMENT, "%s: null pointer", what);
   MKB_REQUIRE(theta > 0.f && theta < INFINITY, MKB_E_ARGUMENT, "%s: theta is not positive", what);
-  status = check(what, qkv, lengths, out, weights, M, q_heads, kv_heads, head_dim, qkv_row_stride, head_dim, dtype, scale, workspace,
-                 workspace_bytes, mkb_paged_attention_workspace_bytes(M, q_heads, kv_heads, head_dim, page, columns, weights != nullptr));
-  if (status != MKB_OK) return status;
-  a.q = qkv; a.positions = positions; a.lengths = lengths; a.k_pages = k_pages; a.v_pages = v_pages; a.out = out; a.weights = weights;
-  a.q_row = qkv_row_stride; a.q_head = head_dim; a.q_heads = q_heads; a.kv_heads = kv_heads; a.rope = 1; a.theta = theta; a.scale = scale;
-  return dispatch(a, M, head_dim, dtype, stream);
+  a.q = qkv; a.positions = positions; a.lengths = lengths; a.q_row = qkv_row_stride; a.q_head = head_dim; a.theta = theta;
+  a.k_pages = static_cast<uint4*>(k_pages); a.v_pages = static_cast<uint4*>(v_pages);
+  return attend(what, a, true, out, weights, M, q_heads, kv_heads, head_dim, page, columns, scale, dtype, workspace, workspace_bytes, stream);
 }

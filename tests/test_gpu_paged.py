@@ -239,6 +239,20 @@ def test_lengths_and_pages_out_of_range_are_left_out(rope):
     assert torch.equal(k_gpu.view(torch.int16), k_before.view(torch.int16))
 
 
+def test_queries_that_are_not_numbers():
+    """A NaN stays with its head, in short sequences and in those that several CTAs share."""
+    lengths = [5, 9000]
+    keys, values, tables, _ = make_cache(lengths, kv_heads=2, head_dim=64, page=16, dtype=HALF)
+    q = torch.randn(2, 8, 64).half().cuda()
+    good, out = torch.empty_like(q), torch.empty_like(q)
+    arguments = (torch.tensor(lengths, dtype=torch.int32).cuda(), keys.cuda(), values.cuda(), tables.cuda())
+    kernels.paged_attention_decode(q, *arguments, good)
+    q[:, 3, 7] = float("nan")
+    kernels.paged_attention_decode(q, *arguments, out)
+    assert torch.isnan(out[:, 3]).all()
+    assert torch.equal(out[:, [0, 1, 2, 4, 5, 6, 7]], good[:, [0, 1, 2, 4, 5, 6, 7]])
+
+
 def test_every_page_out_of_range():
     keys, values, tables, _ = make_cache([40], kv_heads=1, head_dim=64, page=16, dtype=HALF)
     out = torch.full((1, 4, 64), 7.0, dtype=HALF, device="cuda")

@@ -58,9 +58,10 @@ def test_attention_refuses(call):
     for code, changes in (
             (ARGUMENT, [{name: None} for name in ("q", "lengths", "k", "v", "tables", "out")]),
             (ARGUMENT, [{"rows": -1}, {"q_heads": 0}, {"q_heads": 7}, {"kv_heads": 0}, {"page": 0}, {"columns": 0}, {"pages": 0},
-                        {"table_stride": -1}, {"slot_stride": -8}, {"scale": float("nan")}, {"scale": float("inf")}]),
+                        {"workspace": None}, {"size": 1000}, {"table_stride": -1}, {"slot_stride": -8}, {"scale": float("nan")}, {"scale": float("inf")}]),
             (UNSUPPORTED, [{"dtype": F32}, {"dtype": 9}, {"head_dim": 32}, {"head_dim": 96}, {"head_dim": 320}, {"rows": 70000},
                            {"columns": 1 << 20, "page": 1 << 10}, {"pages": 1 << 30, "page_stride": 1 << 20}]),
+            (ARGUMENT, [{"workspace": POINTER + 8}]),
             (ALIGNMENT, [{"q": POINTER + 2}, {"k": POINTER + 8}, {"v": POINTER + 8}, {"out": POINTER + 8}, {"slot_stride": 132},
                          {"page_stride": 4100}, {"head_stride": 2052}, {"q_row": 1028}])):
         for changed in changes:
