@@ -8,10 +8,12 @@
 //   the next leaves partial (max, sum, output) triples, which a second launch joins in the order of the CTAs: the
 //   workspace has two slots per CTA, independent of lengths, and there are no atomics and no state between calls.
 // * A warp copies its own tiles into a ring of its own with cp.async, several tiles ahead, across the borders of
-//   sequences.  A lane copies just those 16-byte pieces that it will itself feed to the tensor core, so that nothing in the
-//   loop waits for another lane's copy: pieces of 8 dimensions of slots g and g + 8 for the keys (g = lane / 4), of slots
-//   2t, 2t + 1, 2t + 8, 2t + 9 for the values (t = lane % 4).  Which dimension stands at which place of the products'
-//   reduction or of their rows is free as long as the queries and the outputs agree.
+//   sequences, and waits for nobody else's.  A copy instruction takes whole rows (rows cut to the 64 bytes that a lane quad
+//   feeds to the tensor core, which would spare the warp its barriers, measured 4.5 TB/s where whole ones measure 5.7).
+//   Pieces of 16 bytes are swapped within 128 bytes by the row so that neither the reads of the keys, pieces t of rows g
+//   (g = lane / 4, t = lane % 4), nor those of the values, pieces g of rows 2t, meet in a bank.  Which dimension stands at
+//   which place of a product's reduction or of its rows is free as long as queries and outputs agree, so a lane feeds the
+//   8 dimensions of a piece to two products and needs no ldmatrix.
 // * Slots are the 16 rows of the tensor core's tile and the group's query heads its 8 columns: S^T = K Q^T, O^T = V^T P^T, so
 //   eight heads leave nothing unused and the running maximum of a column is three shuffles.  P^T turns from the accumulator's
 //   layout to the operand's with movmatrix.  More than eight heads of a group are several tiles of heads, which read the
@@ -62,7 +64,7 @@ template <> struct Types<__half> {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
 };
@@ -75,7 +77,7 @@ template <> struct Types<__nv_bfloat16> {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
   static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
 };
@@ -90,7 +92,7 @@ __device__ __forceinline__ void split(float lo, float hi, uint32_t& pair, uint32
 
 __device__ __forceinline__ uint32_t turn_matrix(uint32_t v) {   // an 8 x 8 matrix of 16-bit values across a warp, transposed
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 
@@ -192,12 +194,16 @@ template <int D> struct Shape {
   static constexpr int kStages = D <= 64 ? 6 : 3;
   static constexpr int kCtas = D <= 128 ? 2 : 1;                 // per SM
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kOps = D / 16;                            // 16-byte pieces a lane copies of the keys, and of the values
-  static constexpr int kStageBytes = 2 * kOps * 32 * 16;
+  static constexpr int kPieces = D / 8;                          // of 16 bytes in a row
+  static constexpr int kOps = kTile * kPieces / 32;              // that a lane copies of the keys, and of the values
+  static constexpr int kHalf = kTile * D * 2;                    // bytes of a tile's keys
+  static constexpr int kStageBytes = 2 * kHalf;
+  static __device__ __forceinline__ int key_at(int row, int piece) { return (row * kPieces + (piece ^ (row & 1) << 2)) * 16; }
+  static __device__ __forceinline__ int value_at(int row, int piece) { return kHalf + (row * kPieces + (piece ^ (row & 6))) * 16; }
   static constexpr int kRowFloats = D + 4;                       // of the outputs where the warps meet
   static constexpr int kRing = 0;
-  static constexpr int kValid = kRing + kWarps * kStages * kStageBytes;     // [warp][stage][lane]: which of a lane's rows count
-  static constexpr int kNorm = kValid + kWarps * kStages * 32 * 4;          // [warp][head] float2
+  static constexpr int kValid = kRing + kWarps * kStages * kStageBytes;     // [warp][stage]: which of a tile's slots count
+  static constexpr int kNorm = kValid + kWarps * kStages * 4;               // [warp][head] float2
   static constexpr int kMeet = kNorm + kWarps * kHeads * 8;                 // [warp]: the stage that holds its outputs
   static constexpr int kTurns = kMeet + kWarps * 4;                         // [D / 2] double: turns per position
   static constexpr int kCosine = kTurns + D / 2 * 8;                        // [D / 2][2] float
@@ -233,8 +239,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
     a.border[cta] = run.begin < run.end && run.tile > 0 ? (int64_t(run.row) * per_row + run.head) : -1;
   if (run.begin >= run.end) return;
 
-  uint8_t* ring = smem + S::kRing + warp * S::kStages * S::kStageBytes + lane * 16;
-  uint32_t* valid_s = reinterpret_cast<uint32_t*>(smem + S::kValid) + warp * S::kStages * 32 + lane;
+  uint8_t* ring = smem + S::kRing + warp * S::kStages * S::kStageBytes;
+  uint32_t* valid_s = reinterpret_cast<uint32_t*>(smem + S::kValid) + warp * S::kStages;
   const int own = int(min(run.end - run.begin, int64_t(1) << 30));
   const int mine = own > warp ? (own - warp + S::kWarps - 1) / S::kWarps : 0;   // tiles of this warp
 
@@ -263,26 +269,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       }
       const int stage = issued % S::kStages;
       const uint32_t to = shared_address(ring + stage * S::kStageBytes);
-      const uint32_t rows[6] = {__shfl_sync(0xffffffffu, offset, g),         __shfl_sync(0xffffffffu, offset, g + 8),
-                                __shfl_sync(0xffffffffu, offset, 2 * t),     __shfl_sync(0xffffffffu, offset, 2 * t + 1),
-                                __shfl_sync(0xffffffffu, offset, 2 * t + 8), __shfl_sync(0xffffffffu, offset, 2 * t + 9)};
-      valid_s[stage * 32] = uint32_t(rows[0] != kNoSlot) | uint32_t(rows[1] != kNoSlot) << 1;
+      const uint32_t counts = __ballot_sync(0xffffffffu, offset != kNoSlot) & 0xffffu;
+      if (lane == 0) valid_s[stage] = counts;
       // a slot that does not count is filled with zeros: whatever lies there, a NaN too, stays out of the products
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint32_t size = rows[r] != kNoSlot ? 16u : 0u;
-        const uint4* from = a.k_pages + (size ? int64_t(rows[r]) + t : 0);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (2 * j + r) * 512), "l"(from + (size ? 4 * j : 0)), "r"(size) : "memory");
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint32_t size = rows[2 + r] != kNoSlot ? 16u : 0u;
-        const uint4* from = a.v_pages + (size ? int64_t(rows[2 + r]) + g : 0);
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (S::kOps + 4 * j + r) * 512), "l"(from + (size ? 8 * j : 0)), "r"(size) : "memory");
+      for (int i = 0; i < S::kOps; ++i) {
+        const int row = (i * 32 + lane) / S::kPieces, piece = (i * 32 + lane) % S::kPieces;
+        const uint32_t source = __shfl_sync(0xffffffffu, offset, row), size = source != kNoSlot ? 16u : 0u;
+        const int64_t from = int64_t(size ? source : 0u) + piece;       // not read where nothing is copied
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + S::key_at(row, piece)), "l"(a.k_pages + from), "r"(size) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + S::value_at(row, piece)), "l"(a.v_pages + from), "r"(size) : "memory");
       }
       if (++issued < mine) {
         ahead.advance(a, per_row, S::kWarps);
@@ -361,45 +357,40 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
     const int skip = int((done - run.begin) % S::kWarps);
     for (int i = warp >= skip ? warp - skip : warp - skip + S::kWarps; i < count; i += S::kWarps) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-      issue();     // into the stage of the tile before, whose pieces the products have taken
+      __syncwarp();   // every lane's copies of this tile are there, and every lane has read the tile before
+      issue();        // into the stage of the tile before
       const int stage = taken++ % S::kStages;
       uint8_t* from = ring + stage * S::kStageBytes;
-      uint32_t valid = valid_s[stage * 32];
+      uint32_t valid = valid_s[stage];
       const int tile = at.tile + i;
       if (Rope && at.extent.added && tile == at.extent.held / kTile) {
-        // the token that this call adds: the lanes that hold pieces of its row put them into their rings and the cache
+        // the token that this call adds goes into the ring, and into the cache
         const int r = at.extent.held % kTile;
         const uint32_t slot = a.layout.vector_of(a.layout.tables + int64_t(at.row) * a.layout.table_stride, kv, at.extent.held);
-        const bool store = slot != kNoSlot && at.head == kv * a.head_tiles;
         if (slot == kNoSlot) {
-          atomicOr(&g_paged_attention_status, 1u);
+          if (lane == 0) atomicOr(&g_paged_attention_status, 1u);
         } else {
-          if ((r & 7) == g) {
-            const uint4* k = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + kv) * D) + t;
-#pragma unroll
-            for (int j = 0; j < D / 64; ++j) {
-              float x[8], y[8];
-              rotate(__ldg(k + 4 * j), __ldg(k + 4 * (j + D / 64)), 32 * j + 8 * t, x, y);
-              const uint4 low = make_uint4(Y::narrow(x[0], x[1]), Y::narrow(x[2], x[3]), Y::narrow(x[4], x[5]), Y::narrow(x[6], x[7]));
-              const uint4 high = make_uint4(Y::narrow(y[0], y[1]), Y::narrow(y[2], y[3]), Y::narrow(y[4], y[5]), Y::narrow(y[6], y[7]));
-              *reinterpret_cast<uint4*>(from + (2 * j + (r >> 3)) * 512) = low;
-              *reinterpret_cast<uint4*>(from + (2 * (j + D / 64) + (r >> 3)) * 512) = high;
-              if (store) {
-                a.k_pages[int64_t(slot) + 4 * j + t] = low;
-                a.k_pages[int64_t(slot) + 4 * (j + D / 64) + t] = high;
-              }
-            }
-            valid |= 1u << (r >> 3);
-          }
-          if (((r & 7) >> 1) == t) {
-            const uint4* v = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + a.kv_heads + kv) * D) + g;
-#pragma unroll
-            for (int j = 0; j < D / 64; ++j) {
-              const uint4 piece = __ldg(v + 8 * j);
-              *reinterpret_cast<uint4*>(from + (S::kOps + 4 * j + (r >> 3) * 2 + (r & 1)) * 512) = piece;
-              if (store) a.v_pages[int64_t(slot) + 8 * j + g] = piece;
+          const bool store = at.head == kv * a.head_tiles;
+          const uint4* k = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + kv) * D);
+          const uint4* v = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + a.kv_heads + kv) * D);
+          if (lane < S::kPieces / 2) {
+            float x[8], y[8];
+            rotate(__ldg(k + lane), __ldg(k + lane + S::kPieces / 2), 8 * lane, x, y);
+            const uint4 low = make_uint4(Y::narrow(x[0], x[1]), Y::narrow(x[2], x[3]), Y::narrow(x[4], x[5]), Y::narrow(x[6], x[7]));
+            const uint4 high = make_uint4(Y::narrow(y[0], y[1]), Y::narrow(y[2], y[3]), Y::narrow(y[4], y[5]), Y::narrow(y[6], y[7]));
+            *reinterpret_cast<uint4*>(from + S::key_at(r, lane)) = low;
+            *reinterpret_cast<uint4*>(from + S::key_at(r, lane + S::kPieces / 2)) = high;
+            if (store) {
+              a.k_pages[int64_t(slot) + lane] = low;
+              a.k_pages[int64_t(slot) + lane + S::kPieces / 2] = high;
             }
           }
+          if (lane < S::kPieces) {
+            const uint4 piece = __ldg(v + lane);
+            *reinterpret_cast<uint4*>(from + S::value_at(r, lane)) = piece;
+            if (store) a.v_pages[int64_t(slot) + lane] = piece;
+          }
+          valid |= 1u << r;
         }
         __syncwarp();
       }
@@ -407,7 +398,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       float score[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
-        const uint4 x = *reinterpret_cast<const uint4*>(from + (2 * j) * 512), y = *reinterpret_cast<const uint4*>(from + (2 * j + 1) * 512);
+        const uint4 x = *reinterpret_cast<const uint4*>(from + S::key_at(g, 4 * j + t));
+        const uint4 y = *reinterpret_cast<const uint4*>(from + S::key_at(g + 8, 4 * j + t));
         Y::mma(score, x.x, y.x, x.y, y.y, query[j][0], query[j][1]);
         Y::mma(Rope ? score : small, x.z, y.z, x.w, y.w, query[j][2], query[j][3]);
         if constexpr (Rope) {
@@ -416,7 +408,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
         }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) score[e] = valid >> (e >> 1) & 1u ? (score[e] + small[e]) * a.scale_log2 : -INFINITY;
+      for (int e = 0; e < 4; ++e) score[e] = valid >> (g + (e >> 1) * 8) & 1u ? (score[e] + small[e]) * a.scale_log2 : -INFINITY;
       if (a.weights != nullptr) {
         float* to = a.scores + (done + i) * (int64_t(min(a.group, kHeads)) * kTile);
 #pragma unroll
@@ -454,7 +446,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       for (int j = 0; j < D / 64; ++j) {
         uint4 v[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const uint4*>(from + (S::kOps + 4 * j + r) * 512);
+        for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const uint4*>(from + S::value_at(2 * t + (r & 1) + (r >> 1) * 8, 8 * j + g));
         const uint32_t words[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
                                       {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
 #pragma unroll
@@ -474,7 +466,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], step);
     }
     const int free_stage = (taken + S::kStages - 1) % S::kStages;
-    float* out_s = reinterpret_cast<float*>(ring - lane * 16 + free_stage * S::kStageBytes);
+    float* out_s = reinterpret_cast<float*>(ring + free_stage * S::kStageBytes);
     float2* norm_s = reinterpret_cast<float2*>(smem + S::kNorm);
     int* meet_s = reinterpret_cast<int*>(smem + S::kMeet);
     if (lane == 0) meet_s[warp] = S::kRing + (warp * S::kStages + free_stage) * S::kStageBytes;
