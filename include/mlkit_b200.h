@@ -353,21 +353,24 @@ int mkb_argmax(const void* logits, void* best, int M, int64_t width, int64_t row
  * head_dim 64, 128, 192 or 256; any number of query heads per key-value head.  What lies in slots behind a sequence's
  * length is never used.  A length beyond the table, and an entry that is no page of the pool, never become an address:
  * such slots are left out and mkb_decode_status is raised.
- * workspace: mkb_paged_attention_workspace_bytes bytes (16-byte aligned), of no meaning before and after the call; calls
- * that may run at the same time need one each.
+ * state: MKB_PAGED_STATE_BYTES bytes that are zero before the first call that uses them; every call leaves them zero.
+ * workspace: mkb_paged_attention_workspace_bytes bytes (16-byte aligned), of no meaning before and after the call.
+ * Calls that may run at the same time need a state and a workspace each.
  * The reference has neither operator: it leaves attention to `transformers`.
  */
+enum { MKB_PAGED_STATE_BYTES = 8192 };
 int64_t mkb_paged_attention_workspace_bytes(int M, int q_heads, int kv_heads, int head_dim, int page, int columns, int with_weights);
 int mkb_paged_attention_decode(const void* q, const int* lengths, const void* k_pages, const void* v_pages, const int* tables,
                                void* out, float* weights, int M, int q_heads, int kv_heads, int head_dim, int page,
                                int columns, int64_t pages, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
                                int64_t table_stride, int64_t q_row_stride, int64_t q_head_stride, float scale, int dtype,
-                               void* workspace, int64_t workspace_bytes, void* stream);
+                               void* state, void* workspace, int64_t workspace_bytes, void* stream);
 int mkb_paged_rope_attention_decode(const void* qkv, const int* positions, const int* lengths, void* k_pages, void* v_pages,
                                     const int* tables, void* out, float* weights, int M, int q_heads, int kv_heads,
                                     int head_dim, int page, int columns, int64_t pages, int64_t page_stride,
                                     int64_t head_stride, int64_t slot_stride, int64_t table_stride, int64_t qkv_row_stride,
-                                    float theta, float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+                                    float theta, float scale, int dtype, void* state, void* workspace, int64_t workspace_bytes,
+                                    void* stream);
 /*
  * Eviction by accumulated attention weight: of n = lengths[m] slots head h keeps k = min(n, budget): the first `sinks`, the
  * last `recent`, and of the others those with the largest weights (NaN below everything, a tie to the lower slot).

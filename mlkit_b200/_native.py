@@ -43,9 +43,9 @@ SIGNATURES = {
     "mkb_attention_decode": (c_int, [c_void_p] * 5 + [c_int] * 5 + [c_float, c_void_p]),
     "mkb_rope_attention_decode": (c_int, [c_void_p] * 5 + [c_int] * 5 + [c_float, c_float, c_void_p]),
     "mkb_paged_attention_workspace_bytes": (c_int64, [c_int] * 7),
-    "mkb_paged_attention_decode": (c_int, [c_void_p] * 7 + [c_int] * 6 + [c_int64] * 7 + [c_float, c_int, c_void_p, c_int64, c_void_p]),
+    "mkb_paged_attention_decode": (c_int, [c_void_p] * 7 + [c_int] * 6 + [c_int64] * 7 + [c_float, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
     "mkb_paged_rope_attention_decode": (c_int, [c_void_p] * 8 + [c_int] * 6 + [c_int64] * 6
-                                        + [c_float, c_float, c_int, c_void_p, c_int64, c_void_p]),
+                                        + [c_float, c_float, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
     "mkb_paged_evict": (c_int, [c_void_p] * 7 + [c_int] * 6 + [c_int64] * 6 + [c_int] * 3 + [c_void_p]),
     "mkb_adjust_logits": (c_int, [c_void_p] * 13 + [c_int] + [c_int64] * 10 + [c_int, c_int, c_void_p]),
     "mkb_argmax": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p]),

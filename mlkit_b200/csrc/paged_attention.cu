@@ -49,7 +49,7 @@ struct AttentionArguments {
   // workspace
   float* partial;           // [ctas][2][kHeads][head_dim]: of the item a CTA's run begins within, and of the one it ends within
   float2* partial_norm;     // [ctas][2][kHeads]: maximum (in powers of two), sum
-  int64_t* border;          // [ctas]: the item that a CTA's run begins within, -1 when it begins with an item or is empty
+  unsigned int* tickets;    // [ctas][3]: of the groups that begin with a CTA's two partials, of the item that crosses its end
   float* norm;              // [rows][q_heads]: log2 of the softmax's sum, with weights
   float* scores;            // [tiles][min(group, 8)][kTile], with weights
 };
@@ -113,8 +113,10 @@ __device__ __forceinline__ Extent extent_of(const AttentionArguments& a, int m, 
 // The tiles of all sequences, (sequence, head tile, tile) in order, dealt out in equal runs.  `per_row`: head tiles of a
 // sequence; `least`: tiles that a CTA should have.  Returns the CTA's run and the (sequence, head tile, tile) it begins at.
 struct Run {
-  int64_t begin, end, total;
+  int64_t begin, end, total, active;
   int row, head, tile;
+  // the CTA whose run holds a tile
+  __device__ __forceinline__ int holder(int64_t index) const { return int(((index + 1) * active - 1) / total); }
 };
 template <bool Rope, int Threads>
 __device__ __forceinline__ Run find_run(const AttentionArguments& a, int per_row, int least, int cta, int ctas) {
@@ -144,9 +146,9 @@ __device__ __forceinline__ Run find_run(const AttentionArguments& a, int per_row
   before -= own;
   Run run;
   run.total = total * per_row;
-  const int64_t active = min(int64_t(ctas), max(int64_t(1), (run.total + least - 1) / least));
-  run.begin = cta < active ? run.total * cta / active : run.total;
-  run.end = cta < active ? run.total * (cta + 1) / active : run.total;
+  run.active = min(int64_t(ctas), max(int64_t(1), (run.total + least - 1) / least));
+  run.begin = cta < run.active ? run.total * cta / run.active : run.total;
+  run.end = cta < run.active ? run.total * (cta + 1) / run.active : run.total;
   if (run.begin < run.end && before * per_row <= run.begin && run.begin < (before + own) * per_row) {
     int64_t rest = run.begin - before * per_row;
     for (int m = first; m < last; ++m) {
@@ -205,18 +207,84 @@ template <int D> struct Shape {
   static constexpr int kValid = kRing + kWarps * kStages * kStageBytes;     // [warp][stage]: which of a tile's slots count
   static constexpr int kNorm = kValid + kWarps * kStages * 4;               // [warp][head] float2
   static constexpr int kMeet = kNorm + kWarps * kHeads * 8;                 // [warp]: the stage that holds its outputs
-  static constexpr int kTurns = kMeet + kWarps * 4;                         // [D / 2] double: turns per position
+  static constexpr int kTicket = kMeet + kWarps * 4;
+  static constexpr int kTurns = (kTicket + 4 + 15) / 16 * 16;               // [D / 2] double: turns per position
   static constexpr int kCosine = kTurns + D / 2 * 8;                        // [D / 2][2] float
   static constexpr int kBytes = kCosine + D / 2 * 8;
   static_assert(kBytes <= (kCtas == 2 ? 115712 : 232448), "shared memory");
   static_assert(kHeads * kRowFloats * 4 <= kStageBytes, "a warp's outputs fit a stage");
 };
 
+constexpr int kGroup = 16;     // partials joined at a time
+
+// Joins `count` partials of an item, of the CTAs left + first, left + first + step, ... (the tail slot of CTA `left`, the head
+// slots of the others): into the output, or into the slot of the first.
+template <typename T, int D, int Threads>
+__device__ __forceinline__ void join(const AttentionArguments& a, int left, int first, int step, int count, int heads, int64_t out_row, bool final, float2* norm_s) {
+  for (int index = threadIdx.x; index < heads * (D / 4); index += Threads) {
+    const int head = index / (D / 4), d = (index - head * (D / 4)) * 4;
+    auto slot_of = [&](int i) { return (int64_t(left + first + i * step) * 2 + (first + i == 0)) * kHeads + head; };
+    float top = -INFINITY, total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int base = 0; base < count; base += kGroup) {
+      float2 norm[kGroup];
+      float4 v[kGroup];
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        const int64_t slot = slot_of(min(base + i, count - 1));
+        norm[i] = __ldcg(a.partial_norm + slot);
+        v[i] = __ldcg(reinterpret_cast<const float4*>(a.partial + slot * D + d));
+      }
+      float now = top;
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) now = fmaxf(now, norm[i].x);
+      const float fade = total == 0.f ? 0.f : exp2f(top - now);
+      top = now;
+      total *= fade;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] *= fade;
+#pragma unroll
+      for (int i = 0; i < kGroup; ++i) {
+        if (base + i >= count || norm[i].y == 0.f) continue;
+        const float share = exp2f(norm[i].x - now);
+        total += norm[i].y * share;
+        x[0] += v[i].x * share; x[1] += v[i].y * share; x[2] += v[i].z * share; x[3] += v[i].w * share;
+      }
+    }
+    if (final) {
+      const float inverse = total == 0.f ? 0.f : 1.f / total;
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (out_row + head) * D + d) =
+          make_uint2(Types<T>::narrow(x[0] * inverse, x[1] * inverse), Types<T>::narrow(x[2] * inverse, x[3] * inverse));
+      if (a.weights != nullptr && d == 0) a.norm[out_row + head] = top - kShift + log2f(total);
+    } else {
+      *reinterpret_cast<float4*>(a.partial + slot_of(0) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+      if (d == 0) norm_s[head] = make_float2(top, total);
+    }
+  }
+  if (!final) {    // the sums last: the other threads of a head have read them
+    __syncthreads();
+    if (int(threadIdx.x) < heads) a.partial_norm[(int64_t(left + first) * 2 + (first == 0)) * kHeads + threadIdx.x] = norm_s[threadIdx.x];
+  }
+}
+
+// Whether this CTA is the last of `count` to come to a ticket, which is then zero again.  What the others wrote before is
+// there for all threads.
+__device__ __forceinline__ bool last_of(unsigned int* ticket, int count, unsigned int* shared) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    const unsigned int before = atomicAdd(ticket, 1u);
+    if (before == unsigned(count - 1)) *ticket = 0;
+    *shared = before;
+    __threadfence();
+  }
+  __syncthreads();
+  return *shared == unsigned(count - 1);
+}
+
 template <typename T, int D, bool Rope>
 __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_attention_kernel(AttentionArguments a) {
   using S = Shape<D>;
   using Y = Types<T>;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, cta = blockIdx.x;
   const int per_row = a.kv_heads * a.head_tiles;
@@ -226,6 +294,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
     for (int i = threadIdx.x; i < D / 2; i += S::kThreads)
       turns_s[i] = exp2(-log2(double(a.theta)) * double(i) / double(D / 2)) * 0.15915494309189533577;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // only now: what a dependent kernel reads before its own wait, the lengths and tables, is then there
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // rows with nothing to attend to
   for (int m = cta; m < a.rows; m += gridDim.x) {
     bool beyond;
@@ -235,8 +305,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
     }
   }
   const Run run = find_run<Rope, S::kThreads>(a, per_row, S::kWarps, cta, gridDim.x);
-  if (threadIdx.x == 0)
-    a.border[cta] = run.begin < run.end && run.tile > 0 ? (int64_t(run.row) * per_row + run.head) : -1;
   if (run.begin >= run.end) return;
 
   uint8_t* ring = smem + S::kRing + warp * S::kStages * S::kStageBytes;
@@ -288,24 +356,45 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (mine > 0) look_up();
+
+  // ---- the run, item by item.  What an item's beginning reads is fetched while the item before ends.
+  Cursor<Rope> at;
+  at.start(a, run);
+  int64_t done = run.begin;
+  int count, position = 0;
+  uint4 query_raw[D / 32], new_low, new_high, new_value;
+  uint32_t new_slot = kNoSlot;
+  auto fetch = [&]() {
+    count = int(min(int64_t(at.extent.tiles - at.tile), run.end - done));
+    const int kv = at.head / a.head_tiles, first = (at.head - kv * a.head_tiles) * kHeads;
+    const T* source = static_cast<const T*>(a.q) + int64_t(at.row) * a.q_row;
+    const uint4* q = reinterpret_cast<const uint4*>(source + int64_t(kv * a.group + first + g) * a.q_head) + t;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) query_raw[j] = g < a.group - first ? __ldg(q + 4 * j) : make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (Rope) {
+      position = __ldg(a.positions + at.row);
+      // the warp that has the tile of the new token
+      if (at.extent.added && at.tile + count == at.extent.tiles && int((done - run.begin + count - 1) % S::kWarps) == warp) {
+        const uint4* k = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + kv) * D);
+        const uint4* v = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + a.kv_heads + kv) * D);
+        if (lane < S::kPieces / 2) { new_low = __ldg(k + lane); new_high = __ldg(k + lane + S::kPieces / 2); }
+        if (lane < S::kPieces) new_value = __ldg(v + lane);
+        new_slot = a.layout.vector_of(a.layout.tables + int64_t(at.row) * a.layout.table_stride, kv, at.extent.held);
+      }
+    }
+  };
+  fetch();
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) issue();
 
-  // ---- the run, item by item
-  Cursor<Rope> at;
-  at.start(a, run);
   int turned = -1, taken = 0;
-  for (int64_t done = run.begin; done < run.end;) {
-    const int count = int(min(int64_t(at.extent.tiles - at.tile), run.end - done));
-    const int kv = at.head / a.head_tiles, head0 = kv * a.group + (at.head - kv * a.head_tiles) * kHeads;
-    const int heads = min(kHeads, a.group - (at.head - kv * a.head_tiles) * kHeads);
-    const T* source = static_cast<const T*>(a.q) + int64_t(at.row) * a.q_row;
+  for (;;) {
+    const int kv = at.head / a.head_tiles, first = (at.head - kv * a.head_tiles) * kHeads;
+    const int head0 = kv * a.group + first, heads = min(kHeads, a.group - first);
     if (Rope && turned != at.row) {
       turned = at.row;
-      const double position = double(__ldg(a.positions + at.row));
-      __syncthreads();
       for (int i = threadIdx.x; i < D / 2; i += S::kThreads) {
-        const double turns = position * turns_s[i];
+        const double turns = double(position) * turns_s[i];
         float sine, cosine;
         sincospif(2.f * float(turns - rint(turns)), &sine, &cosine);
         cosine_s[i] = make_float2(cosine, sine);
@@ -327,15 +416,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
     // queries: head g, dimensions 32j + 8t ..
     uint32_t query[D / 32][4], rest[Rope ? D / 32 : 1][4];
     {
-      const uint4* q = reinterpret_cast<const uint4*>(source + int64_t(head0 + g) * a.q_head) + t;
-      uint4 raw[D / 32];
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) raw[j] = g < heads ? __ldg(q + 4 * j) : make_uint4(0u, 0u, 0u, 0u);
       if constexpr (Rope) {
 #pragma unroll
         for (int j = 0; j < D / 64; ++j) {
           float x[8], y[8];
-          rotate(raw[j], raw[j + D / 64], 32 * j + 8 * t, x, y);
+          rotate(query_raw[j], query_raw[j + D / 64], 32 * j + 8 * t, x, y);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             split<T>(x[2 * i], x[2 * i + 1], query[j][i], rest[j][i]);
@@ -345,7 +430,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       } else {
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
-          query[j][0] = raw[j].x; query[j][1] = raw[j].y; query[j][2] = raw[j].z; query[j][3] = raw[j].w;
+          query[j][0] = query_raw[j].x; query[j][1] = query_raw[j].y; query[j][2] = query_raw[j].z; query[j][3] = query_raw[j].w;
         }
       }
     }
@@ -366,29 +451,25 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       if (Rope && at.extent.added && tile == at.extent.held / kTile) {
         // the token that this call adds goes into the ring, and into the cache
         const int r = at.extent.held % kTile;
-        const uint32_t slot = a.layout.vector_of(a.layout.tables + int64_t(at.row) * a.layout.table_stride, kv, at.extent.held);
-        if (slot == kNoSlot) {
+        if (new_slot == kNoSlot) {
           if (lane == 0) atomicOr(&g_paged_attention_status, 1u);
         } else {
-          const bool store = at.head == kv * a.head_tiles;
-          const uint4* k = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + kv) * D);
-          const uint4* v = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + a.kv_heads + kv) * D);
+          const bool store = first == 0;
           if (lane < S::kPieces / 2) {
             float x[8], y[8];
-            rotate(__ldg(k + lane), __ldg(k + lane + S::kPieces / 2), 8 * lane, x, y);
+            rotate(new_low, new_high, 8 * lane, x, y);
             const uint4 low = make_uint4(Y::narrow(x[0], x[1]), Y::narrow(x[2], x[3]), Y::narrow(x[4], x[5]), Y::narrow(x[6], x[7]));
             const uint4 high = make_uint4(Y::narrow(y[0], y[1]), Y::narrow(y[2], y[3]), Y::narrow(y[4], y[5]), Y::narrow(y[6], y[7]));
             *reinterpret_cast<uint4*>(from + S::key_at(r, lane)) = low;
             *reinterpret_cast<uint4*>(from + S::key_at(r, lane + S::kPieces / 2)) = high;
             if (store) {
-              a.k_pages[int64_t(slot) + lane] = low;
-              a.k_pages[int64_t(slot) + lane + S::kPieces / 2] = high;
+              a.k_pages[int64_t(new_slot) + lane] = low;
+              a.k_pages[int64_t(new_slot) + lane + S::kPieces / 2] = high;
             }
           }
           if (lane < S::kPieces) {
-            const uint4 piece = __ldg(v + lane);
-            *reinterpret_cast<uint4*>(from + S::value_at(r, lane)) = piece;
-            if (store) a.v_pages[int64_t(slot) + lane] = piece;
+            *reinterpret_cast<uint4*>(from + S::value_at(r, lane)) = new_value;
+            if (store) a.v_pages[int64_t(new_slot) + lane] = new_value;
           }
           valid |= 1u << r;
         }
@@ -482,8 +563,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
         *reinterpret_cast<float4*>(row + 64 * j + 4) = make_float4(out[4 * j + 2][c], out[4 * j + 2][c + 2], out[4 * j + 3][c], out[4 * j + 3][c + 2]);
       }
     }
+    const bool from_start = at.tile == 0, whole = from_start && count == at.extent.tiles;
+    const int64_t begin = done - at.tile, end = begin + at.extent.tiles;      // of the item
+    const int64_t out_row = int64_t(at.row) * a.q_heads + head0;
+    done += count;
+    const bool more = done < run.end;
+    if (more) {
+      at.advance(a, per_row, count);
+      fetch();
+    }
     __syncthreads();
-    const bool from_start = at.tile == 0, to_end = at.tile + count == at.extent.tiles;
     for (int index = threadIdx.x; index < heads * (D / 8); index += S::kThreads) {
       const int head = index / (D / 8), d = (index - head * (D / 8)) * 8;
       float all = -INFINITY, total = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -500,12 +589,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
         x[0] += lo.x * fade; x[1] += lo.y * fade; x[2] += lo.z * fade; x[3] += lo.w * fade;
         x[4] += hi.x * fade; x[5] += hi.y * fade; x[6] += hi.z * fade; x[7] += hi.w * fade;
       }
-      if (from_start && to_end) {
+      if (whole) {
         const float inverse = total == 0.f ? 0.f : 1.f / total;
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (int64_t(at.row) * a.q_heads + head0 + head) * D + d) =
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (out_row + head) * D + d) =
             make_uint4(Y::narrow(x[0] * inverse, x[1] * inverse), Y::narrow(x[2] * inverse, x[3] * inverse),
                        Y::narrow(x[4] * inverse, x[5] * inverse), Y::narrow(x[6] * inverse, x[7] * inverse));
-        if (a.weights != nullptr && d == 0) a.norm[int64_t(at.row) * a.q_heads + head0 + head] = all - kShift + log2f(total);
+        if (a.weights != nullptr && d == 0) a.norm[out_row + head] = all - kShift + log2f(total);
       } else {
         const int64_t slot = (int64_t(cta) * 2 + from_start) * kHeads + head;
         float4* row = reinterpret_cast<float4*>(a.partial + slot * D + d);
@@ -514,64 +603,20 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
         if (d == 0) a.partial_norm[slot] = make_float2(all, total);
       }
     }
-    done += count;
-    if (done < run.end) {
-      at.advance(a, per_row, count);
-      __syncthreads();
+    if (!whole) {
+      const int left = run.holder(begin), parts = run.holder(end - 1) - left + 1;      // the CTAs that the item lies in
+      const int first = (cta - left) / kGroup * kGroup, members = min(kGroup, parts - first);
+      unsigned int* ticket_s = reinterpret_cast<unsigned int*>(smem + S::kTicket);
+      if (last_of(a.tickets + (left + first) * 3 + (first == 0), members, ticket_s)) {
+        const bool final = parts <= kGroup;
+        join<T, D, S::kThreads>(a, left, first, 1, members, heads, out_row, final, norm_s);
+        if (!final && last_of(a.tickets + left * 3 + 2, (parts + kGroup - 1) / kGroup, ticket_s))
+          join<T, D, S::kThreads>(a, left, 0, kGroup, (parts + kGroup - 1) / kGroup, heads, out_row, true, norm_s);
+      }
     }
+    if (!more) break;
+    __syncthreads();
   }
-}
-
-// A block per border between two CTAs and head of a tile: the first border within an item joins all that the item left.
-constexpr int kJoinThreads = 256;
-
-template <typename T, int D, bool Rope>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(AttentionArguments a) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kLanes = D / 4, kParts = kJoinThreads / kLanes;    // threads of one partial, partials at a time
-  __shared__ float4 out_s[kParts][kLanes];
-  __shared__ float sum_s[kParts];
-  const int cta = blockIdx.x + 1, head = blockIdx.y;
-  const int64_t item = a.border[cta];
-  if (item < 0 || a.border[cta - 1] == item) return;
-  const int per_row = a.kv_heads * a.head_tiles, row = int(item / per_row), tile = int(item - int64_t(row) * per_row);
-  const int kv = tile / a.head_tiles, first = (tile - kv * a.head_tiles) * kHeads;
-  if (head >= min(kHeads, a.group - first)) return;
-  int count = 1;     // partials: the tail of the CTA before, and the heads of those that begin within the item
-  for (int i = cta; i < a.ctas; i += kJoinThreads) count += __syncthreads_count(i + threadIdx.x < a.ctas && a.border[min(i + int(threadIdx.x), a.ctas - 1)] == item);
-  auto slot_of = [&](int i) { return (i == 0 ? int64_t(cta - 1) * 2 + 1 : int64_t(cta + i - 1) * 2) * kHeads + head; };
-  float top = -INFINITY;
-  for (int i = threadIdx.x & 31; i < count; i += 32) top = fmaxf(top, a.partial_norm[slot_of(i)].x);
-#pragma unroll
-  for (int step = 16; step; step >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
-  const int part = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  if (part < kParts) {
-#pragma unroll 4
-    for (int i = part; i < count; i += kParts) {
-      const float2 norm = a.partial_norm[slot_of(i)];
-      const float4 v = reinterpret_cast<const float4*>(a.partial + slot_of(i) * D)[lane];
-      const float fade = norm.x > -INFINITY ? exp2f(norm.x - top) : 0.f;
-      sum += norm.y * fade;
-      x.x += v.x * fade; x.y += v.y * fade; x.z += v.z * fade; x.w += v.w * fade;
-    }
-    out_s[part][lane] = x;
-    if (lane == 0) sum_s[part] = sum;
-  }
-  __syncthreads();
-  if (part != 0) return;
-  for (int i = 1; i < kParts; ++i) {
-    const float4 v = out_s[i][lane];
-    x.x += v.x; x.y += v.y; x.z += v.z; x.w += v.w;
-    sum += sum_s[i];
-  }
-  const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t query = int64_t(row) * a.q_heads + kv * a.group + first + head;
-  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + query * D + lane * 4) =
-      make_uint2(Types<T>::narrow(x.x * inverse, x.y * inverse), Types<T>::narrow(x.z * inverse, x.w * inverse));
-  if (a.weights != nullptr && lane == 0) a.norm[query] = top - kShift + log2f(sum);
 }
 
 // acc[slot] += the weights of the group's heads, from the scores that the first launch left.  A half warp per tile of 16
@@ -581,12 +626,13 @@ constexpr int kWeightThreads = 256;
 template <bool Rope>
 __global__ void __launch_bounds__(kWeightThreads) paged_weight_kernel(AttentionArguments a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // lengths and tables are there: the kernel before lets this one begin only after its own wait
   constexpr int kParts = kWeightThreads / kTile;
   const Run run = find_run<Rope, kWeightThreads>(a, a.kv_heads, kParts, blockIdx.x, gridDim.x);
-  if (run.begin >= run.end) return;
+  const bool idle = threadIdx.x / kTile >= run.end - run.begin;
+  if (idle) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (idle) return;
   const int part = threadIdx.x / kTile, lane = threadIdx.x % kTile, stored = min(a.group, kHeads);
-  if (part >= run.end - run.begin) return;
   Cursor<Rope> at;
   at.start(a, run);
   int64_t before = run.begin - (int64_t(at.head) * at.extent.tiles + at.tile);      // tiles of the rows before
@@ -598,24 +644,26 @@ __global__ void __launch_bounds__(kWeightThreads) paged_weight_kernel(AttentionA
       before += int64_t(extent_of<Rope>(a, row, beyond).tiles) * a.kv_heads;
     }
   };
+  bool waited = false;
   for (int64_t done = run.begin + part;;) {
     catch_up();
     const int slot = at.tile * kTile + lane;
     const int* table = a.layout.tables + int64_t(at.row) * a.layout.table_stride;
-    if (slot < at.extent.held + at.extent.added) {
-      const int64_t to = a.layout.weight_of(table, a.kv_heads, at.head, slot);
-      if (to >= 0) {
-        const bool added = slot == at.extent.held;
-        float total = 0.f;
-        for (int tile = 0; tile < a.head_tiles; ++tile) {
-          // the scores lie in the order of the first launch: (row, head, head tile, tile)
-          const int64_t from = before * a.head_tiles + (int64_t(at.head) * a.head_tiles + tile) * at.extent.tiles + at.tile;
-          const int heads = min(kHeads, a.group - tile * kHeads);
-          const float* norm = a.norm + int64_t(at.row) * a.q_heads + at.head * a.group + tile * kHeads;
-          for (int h = 0; h < heads; ++h) total += exp2f(a.scores[(from * stored + h) * kTile + lane] - norm[h]);
-        }
-        a.weights[to] = added ? total : a.weights[to] + total;
+    const int64_t to = slot < at.extent.held + at.extent.added ? a.layout.weight_of(table, a.kv_heads, at.head, slot) : -1;
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    waited = true;
+    if (to >= 0) {
+      float total = 0.f;
+      const float held = slot == at.extent.held ? 0.f : a.weights[to];     // the slot of a new token begins at zero
+      for (int tile = 0; tile < a.head_tiles; ++tile) {
+        // the scores lie in the order of the first launch: (row, head, head tile, tile)
+        const int64_t from = before * a.head_tiles + (int64_t(at.head) * a.head_tiles + tile) * at.extent.tiles + at.tile;
+        const int heads = min(kHeads, a.group - tile * kHeads);
+        const float* norm = a.norm + int64_t(at.row) * a.q_heads + at.head * a.group + tile * kHeads;
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) total += h < heads ? exp2f(a.scores[(from * stored + h) * kTile + lane] - norm[h]) : 0.f;
       }
+      a.weights[to] = held + total;
     }
     done += kParts;
     if (done >= run.end) break;
@@ -628,14 +676,14 @@ int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 // CTAs of the first launch, and where the parts of its workspace begin.
 struct Workspace {
   int ctas;
-  int64_t partial, partial_norm, border, norm, scores, bytes;
+  int64_t partial, partial_norm, norm, scores, bytes;
   Workspace(int rows, int q_heads, int kv_heads, int head_dim, int page, int columns, bool weights) {
     ctas = device_info().sm_count * (head_dim <= 128 ? 2 : 1);
     const int group = q_heads / kv_heads, head_tiles = (group + kHeads - 1) / kHeads;
+    if (ctas > MKB_PAGED_STATE_BYTES / 12) ctas = MKB_PAGED_STATE_BYTES / 12;      // three tickets each
     partial = 0;
     partial_norm = partial + aligned(int64_t(ctas) * 2 * kHeads * head_dim * 4);
-    border = partial_norm + aligned(int64_t(ctas) * 2 * kHeads * 8);
-    norm = border + aligned(int64_t(ctas) * 8);
+    norm = partial_norm + aligned(int64_t(ctas) * 2 * kHeads * 8);
     scores = norm + (weights ? aligned(int64_t(rows) * q_heads * 4) : 0);
     const int64_t tiles = int64_t(rows) * kv_heads * head_tiles * ((int64_t(columns) * page + kTile - 1) / kTile);
     bytes = scores + (weights ? aligned(tiles * (group < kHeads ? group : kHeads) * kTile * 4) : 0);
@@ -654,8 +702,6 @@ int launch(AttentionArguments& a, void* stream) {
     opted.fetch_or(uint64_t(1) << (device & 63), std::memory_order_release);
   }
   cudaError_t launched = launch_dependent(paged_attention_kernel<T, D, Rope>, dim3(a.ctas), dim3(S::kThreads), S::kBytes, stream, a);
-  if (launched == cudaSuccess)
-    launched = launch_dependent(paged_join_kernel<T, D, Rope>, dim3(a.ctas - 1, a.group < kHeads ? a.group : kHeads), dim3(kJoinThreads), 0, stream, a);
   if (launched == cudaSuccess && a.weights != nullptr)
     launched = launch_dependent(paged_weight_kernel<Rope>, dim3(a.ctas * 2), dim3(kWeightThreads), 0, stream, a);
   if (launched != cudaSuccess) return cuda_fail(launched, "paged attention launch");
@@ -674,7 +720,7 @@ int dispatch(AttentionArguments& a, int head_dim, void* stream) {
 
 // Checks what both entry points share, fills the rest of `a` and launches.
 int attend(const char* what, AttentionArguments& a, bool rope, void* out, float* weights, int M, int q_heads, int kv_heads, int head_dim,
-           int page, int columns, float scale, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+           int page, int columns, float scale, int dtype, void* state, void* workspace, int64_t workspace_bytes, void* stream) {
   MKB_REQUIRE(a.q && a.lengths && out && (a.positions || !rope), MKB_E_ARGUMENT, "%s: null pointer", what);
   MKB_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0, MKB_E_ARGUMENT, "%s: %d query heads for %d key-value heads", what, q_heads, kv_heads);
   MKB_REQUIRE(dtype == MKB_F16 || dtype == MKB_BF16, MKB_E_UNSUPPORTED, "%s: dtype tag %d (fp16 and bf16 supported)", what, dtype);
@@ -685,13 +731,14 @@ int attend(const char* what, AttentionArguments& a, bool rope, void* out, float*
   const Workspace parts(M, q_heads, kv_heads, head_dim, page, columns, weights != nullptr);
   MKB_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= parts.bytes, MKB_E_ARGUMENT,
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)parts.bytes);
+  MKB_REQUIRE(state != nullptr && (reinterpret_cast<uintptr_t>(state) & 3) == 0, MKB_E_ARGUMENT, "%s: no state", what);
   char* base = static_cast<char*>(workspace);
   a.out = out; a.weights = weights; a.rows = M; a.q_heads = q_heads; a.kv_heads = kv_heads; a.group = q_heads / kv_heads;
   a.head_tiles = (a.group + kHeads - 1) / kHeads; a.ctas = parts.ctas;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.partial = reinterpret_cast<float*>(base + parts.partial);
   a.partial_norm = reinterpret_cast<float2*>(base + parts.partial_norm);
-  a.border = reinterpret_cast<int64_t*>(base + parts.border);
+  a.tickets = static_cast<unsigned int*>(state);
   a.norm = reinterpret_cast<float*>(base + parts.norm);
   a.scores = reinterpret_cast<float*>(base + parts.scores);
   if (dtype == MKB_F16) return rope ? dispatch<__half, true>(a, head_dim, stream) : dispatch<__half, false>(a, head_dim, stream);
@@ -739,8 +786,8 @@ extern "C" int mkb_paged_attention_decode(const void* q, const int* lengths, con
                                           const int* tables, void* out, float* weights, int M, int q_heads, int kv_heads,
                                           int head_dim, int page, int columns, int64_t pages, int64_t page_stride,
                                           int64_t head_stride, int64_t slot_stride, int64_t table_stride, int64_t q_row_stride,
-                                          int64_t q_head_stride, float scale, int dtype, void* workspace, int64_t workspace_bytes,
-                                          void* stream) {
+                                          int64_t q_head_stride, float scale, int dtype, void* state, void* workspace,
+                                          int64_t workspace_bytes, void* stream) {
   using namespace mkb;
   const char* what = "paged_attention_decode";
   MKB_REQUIRE(M >= 0, MKB_E_ARGUMENT, "%s: bad shape", what);
@@ -751,15 +798,15 @@ extern "C" int mkb_paged_attention_decode(const void* q, const int* lengths, con
   if (status != MKB_OK) return status;
   a.q = q; a.lengths = lengths; a.q_row = q_row_stride; a.q_head = q_head_stride;
   a.k_pages = static_cast<uint4*>(const_cast<void*>(k_pages)); a.v_pages = static_cast<uint4*>(const_cast<void*>(v_pages));
-  return attend(what, a, false, out, weights, M, q_heads, kv_heads, head_dim, page, columns, scale, dtype, workspace, workspace_bytes, stream);
+  return attend(what, a, false, out, weights, M, q_heads, kv_heads, head_dim, page, columns, scale, dtype, state, workspace, workspace_bytes, stream);
 }
 
 extern "C" int mkb_paged_rope_attention_decode(const void* qkv, const int* positions, const int* lengths, void* k_pages, void* v_pages,
                                                const int* tables, void* out, float* weights, int M, int q_heads, int kv_heads,
                                                int head_dim, int page, int columns, int64_t pages, int64_t page_stride,
                                                int64_t head_stride, int64_t slot_stride, int64_t table_stride, int64_t qkv_row_stride,
-                                               float theta, float scale, int dtype, void* workspace, int64_t workspace_bytes,
-                                               void* stream) {
+                                               float theta, float scale, int dtype, void* state, void* workspace,
+                                               int64_t workspace_bytes, void* stream) {
   using namespace mkb;
   const char* what = "paged_rope_attention_decode";
   MKB_REQUIRE(M >= 0, MKB_E_ARGUMENT, "%s: bad shape", what);
@@ -771,5 +818,5 @@ extern "C" int mkb_paged_rope_attention_decode(const void* qkv, const int* posit
   MKB_REQUIRE(theta > 0.f && theta < INFINITY, MKB_E_ARGUMENT, "%s: theta is not positive", what);
   a.q = qkv; a.positions = positions; a.lengths = lengths; a.q_row = qkv_row_stride; a.q_head = head_dim; a.theta = theta;
   a.k_pages = static_cast<uint4*>(k_pages); a.v_pages = static_cast<uint4*>(v_pages);
-  return attend(what, a, true, out, weights, M, q_heads, kv_heads, head_dim, page, columns, scale, dtype, workspace, workspace_bytes, stream);
+  return attend(what, a, true, out, weights, M, q_heads, kv_heads, head_dim, page, columns, scale, dtype, state, workspace, workspace_bytes, stream);
 }

@@ -567,35 +567,85 @@ def tokens_of_keys(keys: Tensor) -> Tensor:
 
 # ---- operators over a paged cache, and on the logits ----
 
+_raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream builds an object: 3 us of a call
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
 @functools.lru_cache(maxsize=256)
 def _attention_workspace_bytes(index: int, *shape: int) -> int:
     """Of the device that is current, ``index``."""
     return _native.library().mkb_paged_attention_workspace_bytes(*shape)
 
 
-def _check_pages(what: str, device: torch.device, k_pages: Tensor, v_pages: Tensor, weights: Tensor | None,
-                 *tables: Tensor) -> tuple[int, int, int, int, tuple[int, ...]]:
-    """The pool's ``(pages, kv_heads, page, head_dim)`` and the strides of its first three axes."""
-    shape, strides = k_pages.shape, k_pages.stride()
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != strides or v_pages.dtype != k_pages.dtype:
+STATE_BYTES, STATES = 8192, 128     # of the attention over pages: zeroed words of one call at a time; states of a block
+
+
+class _AttentionScratch:
+    """Where the parts of a sequence meet, on one device: a state and a workspace for each.  Calls on one stream run in order and
+    share theirs; the workspace grows to the largest request.  Captured calls may be replayed at any time, so each owns its
+    state for good (8 KB of a block that was cleared before) and has its workspace in the memory of its graph.  Only a call that
+    is captured when no cleared state is left has its graph clear one."""
+
+    def __init__(self) -> None:
+        self.streams: dict[int, tuple[int, Tensor]] = {}
+        self.blocks: list[Tensor] = []
+        self.left: list[int] = []
+
+    def refill(self, index: int) -> None:
+        self.blocks.append(torch.zeros(STATES * STATE_BYTES, dtype=torch.uint8, device=index))
+        torch.cuda.current_stream(index).synchronize()        # other streams will use the states
+        self.left = [self.blocks[-1].data_ptr() + i * STATE_BYTES for i in range(STATES)] + self.left
+
+    def of(self, index: int, stream: int, need: int) -> tuple[int, Tensor]:
+        if torch.cuda.is_current_stream_capturing():
+            workspace = torch.empty(need + STATE_BYTES, dtype=torch.uint8, device=index)
+            if self.left:
+                return self.left.pop(), workspace
+            workspace[need:].zero_()
+            return workspace.data_ptr() + need, workspace
+        if len(self.left) < STATES // 2:
+            self.refill(index)
+        held = self.streams.get(stream)
+        if held is None or held[1].numel() < need:
+            held = self.streams[stream] = (self.left.pop() if held is None else held[0],
+                                           torch.empty(need, dtype=torch.uint8, device=index))
+        return held
+
+
+_attention_scratch: dict[int, _AttentionScratch] = {}
+
+
+def _scratch(index: int, stream: int, need: int) -> tuple[int, Tensor]:
+    held = _attention_scratch.get(index)
+    if held is None:
+        held = _attention_scratch[index] = _AttentionScratch()
+    return held.of(index, stream, need)
+
+
+def _check_pages(what: str, index: int, k_pages: Tensor, v_pages: Tensor, weights: Tensor | None, *tables: Tensor) -> None:
+    """Pools, tables and accumulator of one layout on device ``index``."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != k_pages.stride() or v_pages.dtype != k_pages.dtype:
         raise ValueError(f"{what}: pages of keys and values must share one [pages, kv_heads, page, head_dim] layout and dtype")
-    if strides[3] != 1:
+    if k_pages.stride(3) != 1:
         raise ValueError(f"{what}: the head dimension of the pages must be contiguous")
     for table in tables:
-        if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1 or table.device != device:
-            raise ValueError(f"{what}: page tables are int32 [rows, columns] with contiguous rows on the device of the pages")
-    if weights is not None and (weights.dtype != torch.float32 or weights.shape != shape[:3] or not weights.is_contiguous()
-                                or weights.device != device):
-        raise ValueError(f"{what}: weights are a contiguous fp32 [pages, kv_heads, page] tensor on the device of the pages")
-    if k_pages.device != device or v_pages.device != device:
+        if table.dtype is not torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+            raise ValueError(f"{what}: page tables are int32 [rows, columns] with contiguous rows")
+        if table.get_device() != index:
+            raise ValueError("all tensors of one call must live on one device")
+    if weights is not None and (weights.dtype is not torch.float32 or weights.shape != shape[:3] or not weights.is_contiguous()):
+        raise ValueError(f"{what}: weights are a contiguous fp32 [pages, kv_heads, page] tensor")
+    if k_pages.get_device() != index or v_pages.get_device() != index or (weights is not None and weights.get_device() != index):
         raise ValueError("all tensors of one call must live on one device")
-    return (*shape, strides[:3])
 
 
-def _check_rows(what: str, device: torch.device, rows: int, **vectors: Tensor) -> None:
-    for name, vector in vectors.items():
-        if vector.dtype != torch.int32 or vector.shape != (rows,) or not vector.is_contiguous() or vector.device != device:
-            raise ValueError(f"{what}: {name} must be a contiguous int32 vector of {rows} rows on the device of the pages")
+def _check_rows(what: str, index: int, rows: int, *vectors: Tensor) -> None:
+    for vector in vectors:
+        if vector.dtype is not torch.int32 or vector.dim() != 1 or vector.shape[0] != rows or not vector.is_contiguous():
+            raise ValueError(f"{what}: lengths and positions are contiguous int32 vectors of {rows} rows")
+        if vector.get_device() != index:
+            raise ValueError("all tensors of one call must live on one device")
 
 
 def paged_attention_decode(q: Tensor, lengths: Tensor, k_pages: Tensor, v_pages: Tensor, tables: Tensor, out: Tensor, *,
@@ -604,29 +654,37 @@ def paged_attention_decode(q: Tensor, lengths: Tensor, k_pages: Tensor, v_pages:
     (pools ``[pages, kv_heads, page, head_dim]``, page numbers ``tables`` int32 [rows, columns]) into ``out``.  An empty sequence
     and a row that is not in use (a negative length) give zeros.  ``weights`` (fp32 [pages, kv_heads, page]) adds up every
     slot's softmax weight over the query heads of its group."""
-    what = "paged_attention_decode"
-    if not q.is_cuda:
+    what, index = "paged_attention_decode", q.get_device()
+    if index < 0:
         raise ValueError("mlkit_b200 kernels require CUDA tensors")
-    device, index = q.device, q.get_device()
-    if torch.cuda.current_device() != index:
+    if _current_device() != index:
         with torch.cuda.device(index):
             return paged_attention_decode(q, lengths, k_pages, v_pages, tables, out, scale=scale, weights=weights)
-    pages, kv_heads, page, head_dim, strides = _check_pages(what, device, k_pages, v_pages, weights, tables)
-    if q.dim() != 3 or q.shape[2] != head_dim or q.stride(2) != 1 or q.dtype != k_pages.dtype:
-        raise ValueError(f"{what}: queries are [rows, q_heads, {head_dim}] in the dtype of the pages with contiguous heads")
-    rows, q_heads = q.shape[:2]
-    if out.shape != q.shape and out.shape != (rows, q_heads * head_dim):
-        raise ValueError(f"{what}: the output is [rows, q_heads, head_dim]")
-    if out.dtype != q.dtype or not out.is_contiguous() or out.device != device or tables.shape[0] != rows:
-        raise ValueError(f"{what}: a contiguous output in the dtype of the queries and a row of tables for each row of queries")
-    _check_rows(what, device, rows, lengths=lengths)
-    need = _attention_workspace_bytes(index, rows, q_heads, kv_heads, head_dim, page, tables.shape[1], int(weights is not None))
-    workspace = q.new_empty(need, dtype=torch.uint8)
+    dtype = q.dtype
+    if q.dim() != 3 or k_pages.dtype is not dtype:
+        raise ValueError(f"{what}: queries are [rows, q_heads, head_dim] in the dtype of the pages")
+    rows, q_heads, head_dim = q.shape
+    row, head, step = q.stride()
+    _check_pages(what, index, k_pages, v_pages, weights, tables)
+    pages, kv_heads, page, width = k_pages.shape
+    if step != 1 or width != head_dim:
+        raise ValueError(f"{what}: queries have contiguous heads of {width}")
+    if (out.dtype is not dtype or out.numel() != rows * q_heads * head_dim or not out.is_contiguous() or out.get_device() != index
+            or out.dim() < 2 or out.shape[0] != rows):
+        raise ValueError(f"{what}: the output is a contiguous [rows, q_heads, head_dim] in the dtype and on the device of the queries")
+    _check_rows(what, index, rows, lengths)
+    columns = tables.shape[1]
+    if tables.shape[0] != rows:
+        raise ValueError(f"{what}: a row of tables for each row of queries")
+    need = _attention_workspace_bytes(index, rows, q_heads, kv_heads, head_dim, page, columns, weights is not None)
+    stream = _raw_stream(index)
+    state, workspace = _scratch(index, stream, need)
+    by_page, by_head, by_slot, _ = k_pages.stride()
     status = _native.library().mkb_paged_attention_decode(
         q.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), out.data_ptr(),
-        _pointer(weights), rows, q_heads, kv_heads, head_dim, page, tables.shape[1], pages, *strides, tables.stride(0),
-        q.stride(0), q.stride(1), head_dim ** -0.5 if scale is None else scale, _tag(q.dtype, "cache"), workspace.data_ptr(), need,
-        torch.cuda.current_stream().cuda_stream)
+        None if weights is None else weights.data_ptr(), rows, q_heads, kv_heads, head_dim, page, columns, pages, by_page, by_head,
+        by_slot, tables.stride(0), row, head, head_dim ** -0.5 if scale is None else scale, _tag(dtype, "cache"),
+        state, workspace.data_ptr(), need, stream)
     if status:
         _native.check(status, what)
 
@@ -638,32 +696,39 @@ def paged_rope_attention_decode(qkv: Tensor, positions: Tensor, lengths: Tensor,
     stored with its value in slot ``lengths`` of the sequence, and the rotated queries attend to slots ``0..lengths``.  ``qkv`` is
     left unrotated, ``lengths`` as they are; a row with a negative length is not in use (zeros, nothing stored).  Positions
     and lengths differ where slots were evicted.  ``weights`` as in ``paged_attention_decode``; a new slot begins at zero."""
-    what = "paged_rope_attention_decode"
-    if not qkv.is_cuda:
+    what, index = "paged_rope_attention_decode", qkv.get_device()
+    if index < 0:
         raise ValueError("mlkit_b200 kernels require CUDA tensors")
-    device, index = qkv.device, qkv.get_device()
-    if torch.cuda.current_device() != index:
+    if _current_device() != index:
         with torch.cuda.device(index):
             return paged_rope_attention_decode(qkv, positions, lengths, k_pages, v_pages, tables, out, q_heads=q_heads,
                                                kv_heads=kv_heads, head_dim=head_dim, theta=theta, scale=scale, weights=weights)
-    pages, heads, page, width, strides = _check_pages(what, device, k_pages, v_pages, weights, tables)
-    if heads != kv_heads or width != head_dim:
-        raise ValueError(f"{what}: pages of {heads} heads of {width}, asked for {kv_heads} of {head_dim}")
-    if qkv.dim() != 2 or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim or qkv.stride(1) != 1 or qkv.dtype != k_pages.dtype:
-        raise ValueError(f"{what}: q | k | v is [rows, {(q_heads + 2 * kv_heads) * head_dim}] in the dtype of the pages")
-    rows = qkv.shape[0]
-    if out.shape != (rows, q_heads * head_dim) and out.shape != (rows, q_heads, head_dim):
-        raise ValueError(f"{what}: the output is [rows, q_heads, head_dim]")
-    if out.dtype != qkv.dtype or not out.is_contiguous() or out.device != device or tables.shape[0] != rows:
-        raise ValueError(f"{what}: a contiguous output in the dtype of the queries and a row of tables for each row of queries")
-    _check_rows(what, device, rows, positions=positions, lengths=lengths)
-    need = _attention_workspace_bytes(index, rows, q_heads, kv_heads, head_dim, page, tables.shape[1], int(weights is not None))
-    workspace = qkv.new_empty(need, dtype=torch.uint8)
+    dtype = qkv.dtype
+    if qkv.dim() != 2 or k_pages.dtype is not dtype:
+        raise ValueError(f"{what}: q | k | v is [rows, (q_heads + 2 * kv_heads) * head_dim] in the dtype of the pages")
+    rows, width = qkv.shape
+    row, step = qkv.stride()
+    _check_pages(what, index, k_pages, v_pages, weights, tables)
+    pages, heads, page, depth = k_pages.shape
+    if step != 1 or heads != kv_heads or depth != head_dim or width != (q_heads + 2 * kv_heads) * head_dim:
+        raise ValueError(f"{what}: rows of {width} values and pages of {heads} heads of {depth} are not {q_heads} query and "
+                         f"{kv_heads} key-value heads of {head_dim}")
+    if (out.dtype is not dtype or out.numel() != rows * q_heads * head_dim or not out.is_contiguous() or out.get_device() != index
+            or out.dim() < 2 or out.shape[0] != rows):
+        raise ValueError(f"{what}: the output is a contiguous [rows, q_heads, head_dim] in the dtype and on the device of the queries")
+    _check_rows(what, index, rows, positions, lengths)
+    columns = tables.shape[1]
+    if tables.shape[0] != rows:
+        raise ValueError(f"{what}: a row of tables for each row of queries")
+    need = _attention_workspace_bytes(index, rows, q_heads, kv_heads, head_dim, page, columns, weights is not None)
+    stream = _raw_stream(index)
+    state, workspace = _scratch(index, stream, need)
+    by_page, by_head, by_slot, _ = k_pages.stride()
     status = _native.library().mkb_paged_rope_attention_decode(
         qkv.data_ptr(), positions.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(),
-        out.data_ptr(), _pointer(weights), rows, q_heads, kv_heads, head_dim, page, tables.shape[1], pages, *strides,
-        tables.stride(0), qkv.stride(0), theta, head_dim ** -0.5 if scale is None else scale, _tag(qkv.dtype, "cache"),
-        workspace.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+        out.data_ptr(), None if weights is None else weights.data_ptr(), rows, q_heads, kv_heads, head_dim, page, columns, pages,
+        by_page, by_head, by_slot, tables.stride(0), row, theta, head_dim ** -0.5 if scale is None else scale, _tag(dtype, "cache"),
+        state, workspace.data_ptr(), need, stream)
     if status:
         _native.check(status, what)
 
@@ -674,25 +739,27 @@ def evict_pages(k_pages: Tensor, v_pages: Tensor, weights: Tensor, tables: Tenso
     heaviest of the others by ``weights`` (a tie to the lower slot).  They are copied, in slot order, to the pages that
     ``new_tables`` names; these must be named once and be none of ``tables``.  Returns the kept slots, int32 [rows, kv_heads,
     budget], -1 behind the last.  The caller swaps the tables, sets the lengths and frees the old pages."""
-    what = "evict_pages"
-    if not k_pages.is_cuda:
+    what, index = "evict_pages", k_pages.get_device()
+    if index < 0:
         raise ValueError("mlkit_b200 kernels require CUDA tensors")
-    device, index = k_pages.device, k_pages.get_device()
-    if torch.cuda.current_device() != index:
+    if _current_device() != index:
         with torch.cuda.device(index):
             return evict_pages(k_pages, v_pages, weights, tables, lengths, new_tables, budget=budget, sinks=sinks, recent=recent)
-    pages, kv_heads, page, head_dim, strides = _check_pages(what, device, k_pages, v_pages, weights, tables, new_tables)
-    if k_pages.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{what}: cache dtype {k_pages.dtype} is not supported (fp16, bf16)")
-    rows = tables.shape[0]
+    _check_pages(what, index, k_pages, v_pages, weights, tables, new_tables)
+    pages, kv_heads, page, head_dim = k_pages.shape
+    _tag(k_pages.dtype, "cache")
+    if k_pages.dtype is torch.float32:
+        raise ValueError(f"{what}: pages are fp16 or bf16")
+    rows, columns = tables.shape
     if new_tables.shape[0] != rows:
         raise ValueError(f"{what}: a row of new tables for each row of tables")
-    _check_rows(what, device, rows, lengths=lengths)
-    kept = torch.empty((rows, kv_heads, max(budget, 0)), dtype=torch.int32, device=device)
+    _check_rows(what, index, rows, lengths)
+    kept = torch.empty((rows, kv_heads, max(budget, 0)), dtype=torch.int32, device=index)
+    by_page, by_head, by_slot, _ = k_pages.stride()
     status = _native.library().mkb_paged_evict(
         k_pages.data_ptr(), v_pages.data_ptr(), weights.data_ptr(), tables.data_ptr(), lengths.data_ptr(), new_tables.data_ptr(),
-        kept.data_ptr(), rows, kv_heads, head_dim, page, tables.shape[1], new_tables.shape[1], pages, *strides, tables.stride(0),
-        new_tables.stride(0), budget, sinks, recent, torch.cuda.current_stream().cuda_stream)
+        kept.data_ptr(), rows, kv_heads, head_dim, page, columns, new_tables.shape[1], pages, by_page, by_head, by_slot,
+        tables.stride(0), new_tables.stride(0), budget, sinks, recent, _raw_stream(index))
     if status:
         _native.check(status, what)
     return kept
@@ -712,11 +779,10 @@ def adjust_logits(logits: Tensor, *, tokens: Tensor | None = None, lengths: Tens
 
     Ids outside ``offset..offset + width`` (-1 fills a row up) have no effect.  ``best`` (int64 [rows]) receives the words of
     ``argmax_keys`` for the result, ``picked`` (int64 [rows]) its greedy tokens."""
-    what = "adjust_logits"
-    if not logits.is_cuda:
+    what, index = "adjust_logits", logits.get_device()
+    if index < 0:
         raise ValueError("mlkit_b200 kernels require CUDA tensors")
-    device, index = logits.device, logits.get_device()
-    if torch.cuda.current_device() != index:
+    if _current_device() != index:
         with torch.cuda.device(index):
             return adjust_logits(logits, tokens=tokens, lengths=lengths, prompts=prompts, repetition=repetition, frequency=frequency,
                                  presence=presence, bias_tokens=bias_tokens, bias=bias, mask=mask, offset=offset, best=best,
@@ -724,37 +790,45 @@ def adjust_logits(logits: Tensor, *, tokens: Tensor | None = None, lengths: Tens
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise ValueError(f"{what}: logits are [rows, width] with contiguous rows")
     rows, width = logits.shape
+    dtype, row = logits.dtype, logits.stride(0)
     if out is None:
         out = logits
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.stride(1) != 1 or out.device != device:
+    elif out.shape != logits.shape or out.dtype is not dtype or out.stride(1) != 1 or out.get_device() != index:
         raise ValueError(f"{what}: the output matches the logits in shape, dtype and device, with contiguous rows")
+
+    def vector(name: str, given: Tensor | None, kind: torch.dtype) -> int | None:
+        if given is None:
+            return None
+        if given.dtype is not kind or given.dim() != 1 or given.shape[0] != rows or not given.is_contiguous() or given.get_device() != index:
+            raise ValueError(f"{what}: {name} must be a contiguous {kind} vector of {rows} rows on the device of the logits")
+        return given.data_ptr()
+
+    def table(name: str, given: Tensor | None, *kinds: torch.dtype) -> tuple[int | None, int, int]:
+        if given is None:
+            return None, 0, 0
+        if given.dim() != 2 or given.shape[0] != rows or given.dtype not in kinds or given.get_device() != index:
+            raise ValueError(f"{what}: {name} must be {kinds[0]} [rows, entries] on the device of the logits")
+        stride, step = given.stride()
+        if step != 1 and given.shape[1] > 1:
+            raise ValueError(f"{what}: {name} must have contiguous rows")
+        return given.data_ptr(), given.shape[1], stride
+
+    history, held, history_stride = table("tokens", tokens, torch.int64, torch.int32)
     if (tokens is None) != (lengths is None):
         raise ValueError(f"{what}: a history needs its lengths")
     if tokens is None and not (prompts is None and repetition is None and frequency is None and presence is None):
         raise ValueError(f"{what}: penalties need a history of tokens")
-    if (bias_tokens is None) != (bias is None) or (bias is not None and bias.shape != bias_tokens.shape):
-        raise ValueError(f"{what}: biases need a token for every value")
-    for name, table, dtypes in (("tokens", tokens, (torch.int32, torch.int64)), ("bias_tokens", bias_tokens, (torch.int32,)),
-                                ("bias", bias, (torch.float32,)), ("mask", mask, (torch.int32,))):
-        if table is not None and (table.dim() != 2 or table.shape[0] != rows or table.dtype not in dtypes or table.device != device
-                                  or (table.stride(1) != 1 and table.shape[1] > 1)):
-            raise ValueError(f"{what}: {name} must be [rows, entries] of {dtypes[0]} with contiguous rows on the device of the logits")
-    for name, vector, dtype in (("lengths", lengths, torch.int32), ("prompts", prompts, torch.int32),
-                                ("repetition", repetition, torch.float32), ("frequency", frequency, torch.float32),
-                                ("presence", presence, torch.float32), ("best", best, torch.int64), ("picked", picked, torch.int64)):
-        if vector is not None and (vector.dtype != dtype or vector.shape != (rows,) or not vector.is_contiguous()
-                                   or vector.device != device):
-            raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector of {rows} rows on the device of the logits")
-    if bias is not None and bias.stride(0) != bias_tokens.stride(0):
-        raise ValueError(f"{what}: biases and their tokens must share a layout")
+    entries, biases, bias_stride = table("bias_tokens", bias_tokens, torch.int32)
+    values, count, stride = table("bias", bias, torch.float32)
+    if (bias is None) != (bias_tokens is None) or count != biases or stride != bias_stride:
+        raise ValueError(f"{what}: biases need a token for every value, in the same layout")
+    bits, words, mask_stride = table("mask", mask, torch.int32)
     status = _native.library().mkb_adjust_logits(
-        logits.data_ptr(), out.data_ptr(), _pointer(tokens), _pointer(lengths), _pointer(prompts), _pointer(repetition),
-        _pointer(frequency), _pointer(presence), _pointer(bias_tokens), _pointer(bias), _pointer(mask), _pointer(best),
-        _pointer(picked), rows, width, logits.stride(0), out.stride(0), 0 if tokens is None else tokens.shape[1],
-        0 if tokens is None else tokens.stride(0), 0 if bias is None else bias.shape[1], 0 if bias is None else bias.stride(0),
-        0 if mask is None else mask.shape[1], 0 if mask is None else mask.stride(0), offset,
-        int(tokens is not None and tokens.dtype == torch.int64), _tag(logits.dtype, "logit"),
-        torch.cuda.current_stream().cuda_stream)
+        logits.data_ptr(), out.data_ptr(), history, vector("lengths", lengths, torch.int32), vector("prompts", prompts, torch.int32),
+        vector("repetition", repetition, torch.float32), vector("frequency", frequency, torch.float32),
+        vector("presence", presence, torch.float32), entries, values, bits, vector("best", best, torch.int64),
+        vector("picked", picked, torch.int64), rows, width, row, out.stride(0), held, history_stride, biases, bias_stride, words,
+        mask_stride, offset, tokens is not None and tokens.dtype is torch.int64, _tag(dtype, "logit"), _raw_stream(index))
     if status:
         _native.check(status, what)
     return out

@@ -12,7 +12,7 @@ needs_no_device = pytest.mark.skipif(torch.cuda.is_available(), reason="an accep
 
 READ = dict(q=POINTER, lengths=POINTER, k=POINTER, v=POINTER, tables=POINTER, out=POINTER, weights=None, rows=2, q_heads=8, kv_heads=2,
             head_dim=128, page=16, columns=4, pages=10, page_stride=2 * 16 * 128, head_stride=16 * 128, slot_stride=128,
-            table_stride=4, q_row=8 * 128, q_head=128, scale=0.1, dtype=F16, workspace=POINTER, size=1 << 40, stream=None)
+            table_stride=4, q_row=8 * 128, q_head=128, scale=0.1, dtype=F16, state=POINTER, workspace=POINTER, size=1 << 40, stream=None)
 EVICT = dict(k=POINTER, v=POINTER, weights=POINTER, tables=POINTER, lengths=POINTER, new=POINTER, kept=POINTER, rows=2, kv_heads=2,
              head_dim=128, page=16, columns=4, new_columns=2, pages=10, page_stride=2 * 16 * 128, head_stride=16 * 128, slot_stride=128,
              table_stride=4, new_stride=2, budget=32, sinks=1, recent=4, stream=None)
@@ -58,7 +58,7 @@ def test_attention_refuses(call):
     for code, changes in (
             (ARGUMENT, [{name: None} for name in ("q", "lengths", "k", "v", "tables", "out")]),
             (ARGUMENT, [{"rows": -1}, {"q_heads": 0}, {"q_heads": 7}, {"kv_heads": 0}, {"page": 0}, {"columns": 0}, {"pages": 0},
-                        {"workspace": None}, {"size": 1000}, {"table_stride": -1}, {"slot_stride": -8}, {"scale": float("nan")}, {"scale": float("inf")}]),
+                        {"state": None}, {"state": POINTER + 2}, {"workspace": None}, {"size": 1000}, {"table_stride": -1}, {"slot_stride": -8}, {"scale": float("nan")}, {"scale": float("inf")}]),
             (UNSUPPORTED, [{"dtype": F32}, {"dtype": 9}, {"head_dim": 32}, {"head_dim": 96}, {"head_dim": 320}, {"rows": 70000},
                            {"columns": 1 << 20, "page": 1 << 10}, {"pages": 1 << 30, "page_stride": 1 << 20}]),
             (ARGUMENT, [{"workspace": POINTER + 8}]),
