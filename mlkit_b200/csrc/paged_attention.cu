@@ -82,6 +82,13 @@ template <> struct Types<__nv_bfloat16> {
   }
 };
 
+// 2^x; below 2^-126 it is 0.  The weights of a softmax and what fades them need no more.
+__device__ __forceinline__ float power_of_two(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Two floats as a pair of 16-bit values and a pair of what their rounding left out.
 template <typename T>
 __device__ __forceinline__ void split(float lo, float hi, uint32_t& pair, uint32_t& rest) {
@@ -110,56 +117,62 @@ __device__ __forceinline__ Extent extent_of(const AttentionArguments& a, int m, 
   return {held, (held + added + kTile - 1) / kTile, added};
 }
 
-// The tiles of all sequences, (sequence, head tile, tile) in order, dealt out in equal runs.  `per_row`: head tiles of a
-// sequence; `least`: tiles that a CTA should have.  Returns the CTA's run and the (sequence, head tile, tile) it begins at.
+// The tiles of all sequences, (sequence, head tile, tile) in order, dealt out in runs that differ by one at most; fewer than
+// 2^31 of them.  `per_row`: head tiles of a sequence; `least`: tiles that a CTA should have.
 struct Run {
-  int64_t begin, end, total, active;
-  int row, head, tile;
+  int begin, end, total;
+  int each, more;                  // tiles of a CTA, and of how many CTAs have one more
+  int row, head, tile;             // where the run begins
   // the CTA whose run holds a tile
-  __device__ __forceinline__ int holder(int64_t index) const { return int(((index + 1) * active - 1) / total); }
+  __device__ __forceinline__ int holder(int index) const {
+    const int longer = more * (each + 1);
+    return index < longer ? index / (each + 1) : more + (index - longer) / each;
+  }
 };
 template <bool Rope, int Threads>
 __device__ __forceinline__ Run find_run(const AttentionArguments& a, int per_row, int least, int cta, int ctas) {
-  __shared__ int64_t warp_s[Threads / 32 + 1];
+  __shared__ int warp_s[Threads / 32];
   __shared__ int found_s[3];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int each = (a.rows + Threads - 1) / Threads;
-  const int first = min(int(threadIdx.x) * each, a.rows), last = min(first + each, a.rows);
+  const int share = (a.rows + Threads - 1) / Threads;
+  const int first = min(int(threadIdx.x) * share, a.rows), last = min(first + share, a.rows);
   bool beyond = false;
-  int64_t own = 0;
+  int own = 0;
   for (int m = first; m < last; ++m) own += extent_of<Rope>(a, m, beyond).tiles;
   if (beyond && cta == 0) atomicOr(&g_paged_attention_status, 1u);
-  int64_t before = own;
+  own *= per_row;
+  int before = own;
 #pragma unroll
   for (int step = 1; step < 32; step <<= 1) {
-    const int64_t other = __shfl_up_sync(0xffffffffu, before, step);
+    const int other = __shfl_up_sync(0xffffffffu, before, step);
     if (lane >= step) before += other;
   }
   if (lane == 31) warp_s[warp] = before;
   __syncthreads();
-  int64_t total = 0;
+  Run run;
+  run.total = 0;
 #pragma unroll
   for (int w = 0; w < Threads / 32; ++w) {
     if (w < warp) before += warp_s[w];
-    total += warp_s[w];
+    run.total += warp_s[w];
   }
   before -= own;
-  Run run;
-  run.total = total * per_row;
-  run.active = min(int64_t(ctas), max(int64_t(1), (run.total + least - 1) / least));
-  run.begin = cta < run.active ? run.total * cta / run.active : run.total;
-  run.end = cta < run.active ? run.total * (cta + 1) / run.active : run.total;
-  if (run.begin < run.end && before * per_row <= run.begin && run.begin < (before + own) * per_row) {
-    int64_t rest = run.begin - before * per_row;
+  const int active = min(ctas, max(1, (run.total + least - 1) / least));
+  run.each = run.total / active;
+  run.more = run.total - run.each * active;
+  run.begin = cta < active ? cta * run.each + min(cta, run.more) : run.total;
+  run.end = cta < active ? run.begin + run.each + (cta < run.more) : run.total;
+  if (run.begin < run.end && before <= run.begin && run.begin < before + own) {
+    int rest = run.begin - before;
     for (int m = first; m < last; ++m) {
-      const int tiles = extent_of<Rope>(a, m, beyond).tiles;
-      if (rest < int64_t(tiles) * per_row) {
+      const Extent extent = extent_of<Rope>(a, m, beyond);
+      if (rest < extent.tiles * per_row) {
         found_s[0] = m;
-        found_s[1] = int(rest / tiles);
-        found_s[2] = int(rest % tiles);
+        found_s[1] = rest / extent.tiles;
+        found_s[2] = rest - found_s[1] * extent.tiles;
         break;
       }
-      rest -= int64_t(tiles) * per_row;
+      rest -= extent.tiles * per_row;
     }
   }
   __syncthreads();
@@ -172,9 +185,10 @@ template <bool Rope>
 struct Cursor {
   int row, head, tile;
   Extent extent;
-  __device__ __forceinline__ void start(const AttentionArguments& a, const Run& run) {
+  // The length is read again (from L1) instead of handed on by find_run: what the compiler then knows of an extent, or
+  // how it schedules the loop for it, measured 15 % of the whole (200 against 233 us for the ragged batch of 64).
+  __device__ __forceinline__ Cursor(const AttentionArguments& a, const Run& run) : row(run.row), head(run.head), tile(run.tile) {
     bool beyond;
-    row = run.row; head = run.head; tile = run.tile;
     extent = extent_of<Rope>(a, row, beyond);
   }
   // `steps` tiles on; the caller keeps it within the run.
@@ -215,54 +229,74 @@ template <int D> struct Shape {
   static_assert(kHeads * kRowFloats * 4 <= kStageBytes, "a warp's outputs fit a stage");
 };
 
-constexpr int kGroup = 16;     // partials joined at a time
+constexpr int kGroup = 8;      // partials joined at a time
 
 // Joins `count` partials of an item, of the CTAs left + first, left + first + step, ... (the tail slot of CTA `left`, the head
-// slots of the others): into the output, or into the slot of the first.
+// slots of the others): into the output, or into the slot of the first.  A thread takes two pieces of four dimensions at a
+// time, so that sixteen loads are under way.
 template <typename T, int D, int Threads>
-__device__ __forceinline__ void join(const AttentionArguments& a, int left, int first, int step, int count, int heads, int64_t out_row, bool final, float2* norm_s) {
-  for (int index = threadIdx.x; index < heads * (D / 4); index += Threads) {
-    const int head = index / (D / 4), d = (index - head * (D / 4)) * 4;
-    auto slot_of = [&](int i) { return (int64_t(left + first + i * step) * 2 + (first + i == 0)) * kHeads + head; };
-    float top = -INFINITY, total = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+__device__ __forceinline__ void join(const AttentionArguments& a, int left, int first, int step, int count, int heads, int64_t out_row, bool final,
+                                     float2* norm_s) {
+  constexpr int kPieces = D / 4;
+  auto slot_of = [&](int i) { return (int64_t(left + first + i * step) * 2 + (first + i == 0)) * kHeads; };
+#pragma unroll 1
+  for (int index = threadIdx.x; index < heads * kPieces; index += 2 * Threads) {
+    float top[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f}, x[2][4] = {};
+    int head[2], d[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int piece = min(index + u * Threads, heads * kPieces - 1);
+      head[u] = piece / kPieces;
+      d[u] = (piece - head[u] * kPieces) * 4;
+    }
+#pragma unroll 1
     for (int base = 0; base < count; base += kGroup) {
-      float2 norm[kGroup];
-      float4 v[kGroup];
+      float2 norm[kGroup][2];
+      float4 v[kGroup][2];
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        const int64_t slot = slot_of(min(base + i, count - 1));
-        norm[i] = __ldcg(a.partial_norm + slot);
-        v[i] = __ldcg(reinterpret_cast<const float4*>(a.partial + slot * D + d));
-      }
-      float now = top;
+      for (int i = 0; i < kGroup; ++i)
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) now = fmaxf(now, norm[i].x);
-      const float fade = total == 0.f ? 0.f : exp2f(top - now);
-      top = now;
-      total *= fade;
+        for (int u = 0; u < 2; ++u) {
+          const int64_t slot = slot_of(min(base + i, count - 1)) + head[u];
+          norm[i][u] = __ldcg(a.partial_norm + slot);
+          v[i][u] = __ldcg(reinterpret_cast<const float4*>(a.partial + slot * D + d[u]));
+        }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] *= fade;
+      for (int u = 0; u < 2; ++u) {
+        float now = top[u];
 #pragma unroll
-      for (int i = 0; i < kGroup; ++i) {
-        if (base + i >= count || norm[i].y == 0.f) continue;
-        const float share = exp2f(norm[i].x - now);
-        total += norm[i].y * share;
-        x[0] += v[i].x * share; x[1] += v[i].y * share; x[2] += v[i].z * share; x[3] += v[i].w * share;
+        for (int i = 0; i < kGroup; ++i) now = fmaxf(now, norm[i][u].x);
+        const float fade = total[u] == 0.f ? 0.f : power_of_two(top[u] - now);
+        top[u] = now;
+        total[u] *= fade;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[u][e] *= fade;
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          if (base + i >= count || norm[i][u].y == 0.f) continue;
+          const float share = power_of_two(norm[i][u].x - now);
+          total[u] += norm[i][u].y * share;
+          x[u][0] += v[i][u].x * share; x[u][1] += v[i][u].y * share; x[u][2] += v[i][u].z * share; x[u][3] += v[i][u].w * share;
+        }
       }
     }
-    if (final) {
-      const float inverse = total == 0.f ? 0.f : 1.f / total;
-      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (out_row + head) * D + d) =
-          make_uint2(Types<T>::narrow(x[0] * inverse, x[1] * inverse), Types<T>::narrow(x[2] * inverse, x[3] * inverse));
-      if (a.weights != nullptr && d == 0) a.norm[out_row + head] = top - kShift + log2f(total);
-    } else {
-      *reinterpret_cast<float4*>(a.partial + slot_of(0) * D + d) = make_float4(x[0], x[1], x[2], x[3]);
-      if (d == 0) norm_s[head] = make_float2(top, total);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (index + u * Threads >= heads * kPieces) continue;
+      if (final) {
+        const float inverse = total[u] == 0.f ? 0.f : 1.f / total[u];
+        *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (out_row + head[u]) * D + d[u]) =
+            make_uint2(Types<T>::narrow(x[u][0] * inverse, x[u][1] * inverse), Types<T>::narrow(x[u][2] * inverse, x[u][3] * inverse));
+        if (a.weights != nullptr && d[u] == 0) a.norm[out_row + head[u]] = top[u] - kShift + log2f(total[u]);
+      } else {
+        *reinterpret_cast<float4*>(a.partial + (slot_of(0) + head[u]) * D + d[u]) = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+        if (d[u] == 0) norm_s[head[u]] = make_float2(top[u], total[u]);
+      }
     }
   }
   if (!final) {    // the sums last: the other threads of a head have read them
     __syncthreads();
-    if (int(threadIdx.x) < heads) a.partial_norm[(int64_t(left + first) * 2 + (first == 0)) * kHeads + threadIdx.x] = norm_s[threadIdx.x];
+    if (int(threadIdx.x) < heads) a.partial_norm[slot_of(0) + threadIdx.x] = norm_s[threadIdx.x];
   }
 }
 
@@ -271,11 +305,10 @@ __device__ __forceinline__ void join(const AttentionArguments& a, int left, int 
 __device__ __forceinline__ bool last_of(unsigned int* ticket, int count, unsigned int* shared) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    __threadfence();
-    const unsigned int before = atomicAdd(ticket, 1u);
+    unsigned int before;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(ticket) : "memory");
     if (before == unsigned(count - 1)) *ticket = 0;
     *shared = before;
-    __threadfence();
   }
   __syncthreads();
   return *shared == unsigned(count - 1);
@@ -296,76 +329,93 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // only now: what a dependent kernel reads before its own wait, the lengths and tables, is then there
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // rows with nothing to attend to
-  for (int m = cta; m < a.rows; m += gridDim.x) {
-    bool beyond;
-    if (extent_of<Rope>(a, m, beyond).tiles == 0) {
+  const Run run = find_run<Rope, S::kThreads>(a, per_row, S::kWarps, cta, gridDim.x);
+  auto clear = [&]() {     // rows with nothing to attend to
+    for (int m = cta; m < a.rows; m += gridDim.x) {
+      bool beyond;
+      if (extent_of<Rope>(a, m, beyond).tiles != 0) continue;
       uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + int64_t(m) * a.q_heads * D);
       for (int i = threadIdx.x; i < a.q_heads * D / 8; i += S::kThreads) out[i] = make_uint4(0u, 0u, 0u, 0u);
     }
+  };
+  if (run.begin >= run.end) {
+    clear();
+    return;
   }
-  const Run run = find_run<Rope, S::kThreads>(a, per_row, S::kWarps, cta, gridDim.x);
-  if (run.begin >= run.end) return;
 
   uint8_t* ring = smem + S::kRing + warp * S::kStages * S::kStageBytes;
   uint32_t* valid_s = reinterpret_cast<uint32_t*>(smem + S::kValid) + warp * S::kStages;
-  const int own = int(min(run.end - run.begin, int64_t(1) << 30));
+  const int own = run.end - run.begin;
   const int mine = own > warp ? (own - warp + S::kWarps - 1) / S::kWarps : 0;   // tiles of this warp
 
   // ---- copies: the page of a tile is looked up one tile before its copies are issued
-  Cursor<Rope> ahead;
-  ahead.start(a, run);
-  if (mine > 0) ahead.advance(a, per_row, warp);
-  uint32_t page_id = 0, inner = 0;
-  bool inside = false;
-  auto look_up = [&]() {     // of lane % 16, the slot of the tile at `ahead`
-    const uint32_t slot = uint32_t(ahead.tile) * kTile + (lane & 15);
-    inside = slot < uint32_t(ahead.extent.held);
-    if (inside) {
-      const uint32_t column = a.layout.page.quotient(slot);
-      page_id = uint32_t(__ldg(a.layout.tables + int64_t(ahead.row) * a.layout.table_stride + column));
-      inner = uint32_t(ahead.head / a.head_tiles) * a.layout.head_stride + (slot - column * a.layout.page.divisor) * a.layout.slot_stride;
-    }
+  Cursor<Rope> ahead(a, run);
+  struct Page {
+    uint32_t id, inner;     // of lane % 16, the slot of a tile: its page, and the 16-byte vectors behind the page's beginning
+    bool inside;
   };
-  int issued = 0;
-  auto issue = [&]() {
+  int looked_up = 0;
+  auto look_up = [&]() {
+    Page page{0u, 0u, false};
+    if (looked_up >= mine) return page;
+    ahead.advance(a, per_row, looked_up == 0 ? warp : S::kWarps);
+    ++looked_up;
+    const uint32_t slot = uint32_t(ahead.tile) * kTile + (lane & 15);
+    page.inside = slot < uint32_t(ahead.extent.held);
+    if (page.inside) {
+      const uint32_t column = a.layout.page.quotient(slot);
+      page.id = uint32_t(__ldg(a.layout.tables + int64_t(ahead.row) * a.layout.table_stride + column));
+      page.inner = uint32_t(ahead.head / a.head_tiles) * a.layout.head_stride + (slot - column * a.layout.page.divisor) * a.layout.slot_stride;
+    }
+    return page;
+  };
+  int issued = 0, into = 0;
+  const uint32_t copies_to = shared_address(ring);
+  auto issue = [&](const Page& page) {
     if (issued < mine) {
       uint32_t offset = kNoSlot;
-      if (inside) {
-        if (page_id < a.layout.pages) offset = page_id * a.layout.page_stride + inner;
+      if (page.inside) {
+        if (page.id < a.layout.pages) offset = page.id * a.layout.page_stride + page.inner;
         else atomicOr(&g_paged_attention_status, 1u);
       }
-      const int stage = issued % S::kStages;
-      const uint32_t to = shared_address(ring + stage * S::kStageBytes);
+      const uint32_t to = copies_to + into * S::kStageBytes;
       const uint32_t counts = __ballot_sync(0xffffffffu, offset != kNoSlot) & 0xffffu;
-      if (lane == 0) valid_s[stage] = counts;
-      // a slot that does not count is filled with zeros: whatever lies there, a NaN too, stays out of the products
+      if (lane == 0) valid_s[into] = counts;
+      into = into + 1 == S::kStages ? 0 : into + 1;
+      if (counts == 0xffffu) {
 #pragma unroll
-      for (int i = 0; i < S::kOps; ++i) {
-        const int row = (i * 32 + lane) / S::kPieces, piece = (i * 32 + lane) % S::kPieces;
-        const uint32_t source = __shfl_sync(0xffffffffu, offset, row), size = source != kNoSlot ? 16u : 0u;
-        const int64_t from = int64_t(size ? source : 0u) + piece;       // not read where nothing is copied
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + S::key_at(row, piece)), "l"(a.k_pages + from), "r"(size) : "memory");
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + S::value_at(row, piece)), "l"(a.v_pages + from), "r"(size) : "memory");
+        for (int i = 0; i < S::kOps; ++i) {
+          const int row = (i * 32 + lane) / S::kPieces, piece = (i * 32 + lane) % S::kPieces;
+          const uint32_t from = __shfl_sync(0xffffffffu, offset, row);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + S::key_at(row, piece)), "l"(a.k_pages + piece + from) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + S::value_at(row, piece)), "l"(a.v_pages + piece + from) : "memory");
+        }
+      } else {
+        // a slot that does not count is filled with zeros: whatever lies there, a NaN too, stays out of the products
+#pragma unroll
+        for (int i = 0; i < S::kOps; ++i) {
+          const int row = (i * 32 + lane) / S::kPieces, piece = (i * 32 + lane) % S::kPieces;
+          const uint32_t from = __shfl_sync(0xffffffffu, offset, row), size = from != kNoSlot ? 16u : 0u;
+          const int64_t source = int64_t(size ? from : 0u) + piece;       // not read where nothing is copied
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + S::key_at(row, piece)), "l"(a.k_pages + source), "r"(size) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + S::value_at(row, piece)), "l"(a.v_pages + source), "r"(size) : "memory");
+        }
       }
-      if (++issued < mine) {
-        ahead.advance(a, per_row, S::kWarps);
-        look_up();
-      }
+      ++issued;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  if (mine > 0) look_up();
+  Page pages[S::kStages - 1];
+#pragma unroll
+  for (int i = 0; i < S::kStages - 1; ++i) pages[i] = look_up();
 
   // ---- the run, item by item.  What an item's beginning reads is fetched while the item before ends.
-  Cursor<Rope> at;
-  at.start(a, run);
-  int64_t done = run.begin;
-  int count, position = 0;
+  Cursor<Rope> at(a, run);
+  int done = run.begin, count, position = 0;
   uint4 query_raw[D / 32], new_low, new_high, new_value;
   uint32_t new_slot = kNoSlot;
   auto fetch = [&]() {
-    count = int(min(int64_t(at.extent.tiles - at.tile), run.end - done));
+    count = min(at.extent.tiles - at.tile, run.end - done);
     const int kv = at.head / a.head_tiles, first = (at.head - kv * a.head_tiles) * kHeads;
     const T* source = static_cast<const T*>(a.q) + int64_t(at.row) * a.q_row;
     const uint4* q = reinterpret_cast<const uint4*>(source + int64_t(kv * a.group + first + g) * a.q_head) + t;
@@ -374,7 +424,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
     if constexpr (Rope) {
       position = __ldg(a.positions + at.row);
       // the warp that has the tile of the new token
-      if (at.extent.added && at.tile + count == at.extent.tiles && int((done - run.begin + count - 1) % S::kWarps) == warp) {
+      if (at.extent.added && at.tile + count == at.extent.tiles && (done - run.begin + count - 1) % S::kWarps == warp) {
         const uint4* k = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + kv) * D);
         const uint4* v = reinterpret_cast<const uint4*>(source + int64_t(a.q_heads + a.kv_heads + kv) * D);
         if (lane < S::kPieces / 2) { new_low = __ldg(k + lane); new_high = __ldg(k + lane + S::kPieces / 2); }
@@ -385,9 +435,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
   };
   fetch();
 #pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) issue();
+  for (int i = 0; i < S::kStages - 1; ++i) issue(pages[i]);
+  Page next = look_up();
+  clear();
 
-  int turned = -1, taken = 0;
+  // where a lane's pieces lie in a stage: of the keys 32j .. and 32j + 32 .. (j even) of row g, of the values of row 2t
+  const int key0 = S::key_at(g, t), key1 = S::key_at(g, t + 4), value0 = S::value_at(2 * t, g);
+  int turned = -1, stage = 0;
   for (;;) {
     const int kv = at.head / a.head_tiles, first = (at.head - kv * a.head_tiles) * kHeads;
     const int head0 = kv * a.group + first, heads = min(kHeads, a.group - first);
@@ -439,14 +493,15 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
     for (int i = 0; i < D / 16; ++i) out[i][0] = out[i][1] = out[i][2] = out[i][3] = 0.f;
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
 
-    const int skip = int((done - run.begin) % S::kWarps);
+    const int skip = (done - run.begin) % S::kWarps;
     for (int i = warp >= skip ? warp - skip : warp - skip + S::kWarps; i < count; i += S::kWarps) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
       __syncwarp();   // every lane's copies of this tile are there, and every lane has read the tile before
-      issue();        // into the stage of the tile before
-      const int stage = taken++ % S::kStages;
+      issue(next);    // into the stage of the tile before
+      next = look_up();
       uint8_t* from = ring + stage * S::kStageBytes;
       uint32_t valid = valid_s[stage];
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
       const int tile = at.tile + i;
       if (Rope && at.extent.added && tile == at.extent.held / kTile) {
         // the token that this call adds goes into the ring, and into the cache
@@ -479,8 +534,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       float score[4] = {0.f, 0.f, 0.f, 0.f}, small[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
-        const uint4 x = *reinterpret_cast<const uint4*>(from + S::key_at(g, 4 * j + t));
-        const uint4 y = *reinterpret_cast<const uint4*>(from + S::key_at(g + 8, 4 * j + t));
+        const uint8_t* key = from + (j & 1 ? key1 : key0) + (j >> 1) * 128;
+        const uint4 x = *reinterpret_cast<const uint4*>(key), y = *reinterpret_cast<const uint4*>(key + 8 * S::kPieces * 16);
         Y::mma(score, x.x, y.x, x.y, y.y, query[j][0], query[j][1]);
         Y::mma(Rope ? score : small, x.z, y.z, x.w, y.w, query[j][2], query[j][3]);
         if constexpr (Rope) {
@@ -489,9 +544,14 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
         }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) score[e] = valid >> (g + (e >> 1) * 8) & 1u ? (score[e] + small[e]) * a.scale_log2 : -INFINITY;
+      for (int e = 0; e < 4; ++e) score[e] = (score[e] + small[e]) * a.scale_log2;
+      if (valid != 0xffffu) {
+        valid >>= g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) score[e] = valid >> (e >> 1) * 8 & 1u ? score[e] : -INFINITY;
+      }
       if (a.weights != nullptr) {
-        float* to = a.scores + (done + i) * (int64_t(min(a.group, kHeads)) * kTile);
+        float* to = a.scores + int64_t(done + i) * (min(a.group, kHeads) * kTile);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (2 * t + (e & 1) < heads) to[(2 * t + (e & 1)) * kTile + g + (e >> 1) * 8] = score[e];
@@ -506,7 +566,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const float now = fmaxf(top[c], high[c]);
-          const float fade = now > -INFINITY ? exp2f(top[c] - now) : 1.f;
+          const float fade = now > -INFINITY ? power_of_two(top[c] - now) : 1.f;
           top[c] = now;
           sum[c] *= fade;
 #pragma unroll
@@ -516,7 +576,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       const float base[2] = {top[0] > -INFINITY ? top[0] - kShift : 0.f, top[1] > -INFINITY ? top[1] - kShift : 0.f};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        score[e] = exp2f(score[e] - base[e & 1]);
+        score[e] = power_of_two(score[e] - base[e & 1]);
         sum[e & 1] += score[e];
       }
       uint32_t p0, p1, r0, r1;
@@ -527,7 +587,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       for (int j = 0; j < D / 64; ++j) {
         uint4 v[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const uint4*>(from + S::value_at(2 * t + (r & 1) + (r >> 1) * 8, 8 * j + g));
+        for (int r = 0; r < 4; ++r) v[r] = *reinterpret_cast<const uint4*>(from + value0 + ((r & 1) + (r >> 1) * 8) * (S::kPieces * 16) + j * 128);
         const uint32_t words[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
                                       {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
 #pragma unroll
@@ -546,7 +606,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], step);
       sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], step);
     }
-    const int free_stage = (taken + S::kStages - 1) % S::kStages;
+    const int free_stage = stage == 0 ? S::kStages - 1 : stage - 1;
     float* out_s = reinterpret_cast<float*>(ring + free_stage * S::kStageBytes);
     float2* norm_s = reinterpret_cast<float2*>(smem + S::kNorm);
     int* meet_s = reinterpret_cast<int*>(smem + S::kMeet);
@@ -564,7 +624,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       }
     }
     const bool from_start = at.tile == 0, whole = from_start && count == at.extent.tiles;
-    const int64_t begin = done - at.tile, end = begin + at.extent.tiles;      // of the item
+    const int begin = done - at.tile, end = begin + at.extent.tiles;          // of the item
     const int64_t out_row = int64_t(at.row) * a.q_heads + head0;
     done += count;
     const bool more = done < run.end;
@@ -582,7 +642,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
       for (int w = 0; w < S::kWarps; ++w) {
         const float2 norm = norm_s[w * kHeads + head];
         if (norm.y == 0.f) continue;            // no tiles, or none whose slots count
-        const float fade = exp2f(norm.x - all);
+        const float fade = power_of_two(norm.x - all);
         total += norm.y * fade;
         const float4* row = reinterpret_cast<const float4*>(smem + meet_s[w] + (head * S::kRowFloats + d) * 4);
         const float4 lo = row[0], hi = row[1];
@@ -633,19 +693,18 @@ __global__ void __launch_bounds__(kWeightThreads) paged_weight_kernel(AttentionA
   if (idle) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (idle) return;
   const int part = threadIdx.x / kTile, lane = threadIdx.x % kTile, stored = min(a.group, kHeads);
-  Cursor<Rope> at;
-  at.start(a, run);
-  int64_t before = run.begin - (int64_t(at.head) * at.extent.tiles + at.tile);      // tiles of the rows before
+  Cursor<Rope> at(a, run);
+  int before = run.begin - (at.head * at.extent.tiles + at.tile);      // tiles of the rows before
   int row = at.row;
   at.advance(a, a.kv_heads, part);
   auto catch_up = [&]() {
     for (; row < at.row; ++row) {
       bool beyond;
-      before += int64_t(extent_of<Rope>(a, row, beyond).tiles) * a.kv_heads;
+      before += extent_of<Rope>(a, row, beyond).tiles * a.kv_heads;
     }
   };
   bool waited = false;
-  for (int64_t done = run.begin + part;;) {
+  for (int done = run.begin + part;;) {
     catch_up();
     const int slot = at.tile * kTile + lane;
     const int* table = a.layout.tables + int64_t(at.row) * a.layout.table_stride;
@@ -657,11 +716,11 @@ __global__ void __launch_bounds__(kWeightThreads) paged_weight_kernel(AttentionA
       const float held = slot == at.extent.held ? 0.f : a.weights[to];     // the slot of a new token begins at zero
       for (int tile = 0; tile < a.head_tiles; ++tile) {
         // the scores lie in the order of the first launch: (row, head, head tile, tile)
-        const int64_t from = before * a.head_tiles + (int64_t(at.head) * a.head_tiles + tile) * at.extent.tiles + at.tile;
+        const int64_t from = before * a.head_tiles + (at.head * a.head_tiles + tile) * at.extent.tiles + at.tile;
         const int heads = min(kHeads, a.group - tile * kHeads);
         const float* norm = a.norm + int64_t(at.row) * a.q_heads + at.head * a.group + tile * kHeads;
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) total += h < heads ? exp2f(a.scores[(from * stored + h) * kTile + lane] - norm[h]) : 0.f;
+        for (int h = 0; h < kHeads; ++h) total += h < heads ? power_of_two(a.scores[(from * stored + h) * kTile + lane] - norm[h]) : 0.f;
       }
       a.weights[to] = held + total;
     }
@@ -728,6 +787,8 @@ int attend(const char* what, AttentionArguments& a, bool rope, void* out, float*
   MKB_REQUIRE(fabsf(scale) < INFINITY, MKB_E_ARGUMENT, "%s: scale is not finite", what);
   MKB_REQUIRE(((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 && a.q_row % 8 == 0 && a.q_head % 8 == 0,
               MKB_E_ALIGNMENT, "%s: queries and outputs lie on 16-byte vectors", what);
+  MKB_REQUIRE(int64_t(M) * kv_heads * ((q_heads / kv_heads + kHeads - 1) / kHeads) * ((int64_t(columns) * page + kTile - 1) / kTile) < (int64_t(1) << 31),
+              MKB_E_UNSUPPORTED, "%s: %d sequences of %d pages of %d slots", what, M, columns, page);
   const Workspace parts(M, q_heads, kv_heads, head_dim, page, columns, weights != nullptr);
   MKB_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= parts.bytes, MKB_E_ARGUMENT,
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)parts.bytes);
