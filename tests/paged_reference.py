@@ -1,6 +1,7 @@
 """Plain 64-bit restatements of the operators over a paged cache and on logits, and the rounding they are held to."""
 
 import math
+from collections import Counter
 
 import torch
 
@@ -81,12 +82,13 @@ def evicted(weight, budget, sinks, recent):
 def adjusted(row, offset, *, history=(), prompt=0, repetition=1.0, frequency=0.0, presence=0.0, biases=(), mask=None):
     """One row of logits in 64 bits."""
     x = row.double().clone()
+    generated = Counter(history[max(prompt, 0):])
     for token in set(history):
         i = token - offset
         if not 0 <= i < x.numel():
             continue
         x[i] = x[i] / repetition if x[i] > 0 else x[i] * repetition
-        count = list(history[max(prompt, 0):]).count(token)
+        count = generated[token]
         x[i] -= frequency * count + (presence if count else 0.0)
     for token, value in biases:
         if 0 <= token - offset < x.numel():

@@ -85,9 +85,48 @@ def test_histories_biases_and_masks_alone(history, biases, masked):
     check(4, 2000, 0, 2000, history, biases, masked, torch.bfloat16, long=False)
 
 
+@pytest.mark.parametrize("rows,vocab,history,biases", [(2, 20000, 6144, 0), (2, 20000, 6000, 145), (3, 30011, 20000, 700), (1, 140000, 9000, 0)])
+def test_histories_beyond_the_table(rows, vocab, history, biases):
+    """More tokens than the hash table of a CTA takes, and as many as it just takes."""
+    check(rows, vocab, 0, vocab, history, biases, False, torch.float32)
+
+
+def test_a_table_full_of_different_tokens():
+    """6144 different tokens, the most of a table, in one slice and over several; and 6145."""
+    for history, step in ((6144, 1), (6144, 3), (6145, 1)):
+        tokens = (torch.arange(history) * step).view(1, -1)
+        width = int(tokens.max()) + 10
+        logits = torch.randn(1, width, generator=torch.Generator().manual_seed(0))
+        out = kernels.adjust_logits(logits.cuda(), tokens=tokens.cuda(), lengths=torch.tensor([history], dtype=torch.int32).cuda(),
+                                    presence=torch.tensor([2.0]).cuda())
+        expected = logits.clone()
+        expected[0, tokens[0]] -= 2.0
+        assert torch.equal(out.cpu(), expected)
+
+
 @pytest.mark.parametrize("rows", [1, 9, 200])
 def test_in_place_and_batches(rows):
     check(rows, 3000, 0, 3000, 64, 4, True, torch.float16, in_place=True, long=rows == 9)
+
+
+def test_biases_of_one_token_many_times():
+    """1500 entries of three tokens: added up in their order in 64 bits, whichever threads meet them."""
+    entries = torch.randint(0, 3, (2, 1500), generator=torch.Generator().manual_seed(0)) * 400 + 17
+    values = torch.randn(2, 1500, generator=torch.Generator().manual_seed(1)) * 100
+    logits = torch.zeros(2, 1000, device="cuda")
+    outs = [kernels.adjust_logits(logits.clone(), bias_tokens=entries.int().cuda(), bias=values.cuda()) for _ in range(5)]
+    expected = torch.zeros(2, 1000, dtype=torch.float64).scatter_add_(1, entries, values.double()).float()
+    for out in outs:
+        assert torch.equal(out.cpu(), expected)
+
+
+def test_zeros_of_both_signs_tie():
+    logits = torch.full((3, 5000), -1.0)
+    logits[0, 700], logits[0, 701], logits[1, 4000], logits[1, 4999], logits[2, 3] = -0.0, 0.0, 0.0, -0.0, -0.0
+    for dtype in DTYPES:
+        picked = torch.zeros(3, dtype=torch.int64, device="cuda")
+        kernels.adjust_logits(logits.to(dtype).cuda(), picked=picked)
+        assert picked.tolist() == [700, 4000, 3]
 
 
 def test_one_token_many_times():
