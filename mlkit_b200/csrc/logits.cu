@@ -27,7 +27,7 @@ struct LogitArguments {
   unsigned long long* best;
   long long* picked;
   int64_t logits_stride, out_stride, tokens_stride, bias_stride, mask_words, mask_stride, offset;
-  int width, history, biases, long_tokens, slice, chunk;
+  int width, history, biases, long_tokens, slice, chunk, slots;
 };
 
 // What bounds it: for many rows the logits, read and written once (4 bytes a token in 16 bits); for few, the chain of
@@ -37,17 +37,19 @@ struct LogitArguments {
 // under way.  Then the slice passes in 16-byte pieces as it is, masked in its own type, but for the marked tokens, and the
 // greedy pick looks at a piece's maximum only; the marked tokens follow from the table's list, one a thread.  The CTAs' best
 // words meet in the first one's shared memory, since an order of (value, lower token) does not depend on who comes first.
-// Tried for 128 rows of 128256 tokens with 4000 in the history, 300 biases and a mask: penalties worked out where a piece
+// Measured for 128 rows of 128256 tokens with 4000 in the history, 300 biases and a mask: penalties worked out where a piece
 // met them 115 us (almost every warp did all of it for all of its tokens), a count per token in shared memory, chunk by chunk,
 // 77 us, counts of the history's shares added into the other CTAs' memory 96 us (common tokens queued there).
 constexpr int kLogitThreads = 512;
-constexpr int kDeep = 4;                  // pieces of a thread under way
-constexpr int kSlots = 8192;              // of the hash table
-constexpr int kMost = 6144;               // tokens it takes; more history than that goes by chunks of that many tokens
+constexpr int kDeep = 2;                  // pieces of a thread under way
+constexpr int kSlots = 8192;              // of the hash table, at most; a power of two
+constexpr int kMost = 6144;               // tokens it takes, three quarters of its slots; more history than that goes by chunks of that many tokens
 constexpr int kRanks = 16;                // CTAs of a row, at most
 constexpr uint32_t kSeen = 0x80000000u;   // of a count: the token is in the prompt
 constexpr uint32_t kBiased = 0x40000000u; // of a count: the token has a bias
 constexpr uint32_t kCount = kBiased - 1;  // how often it was generated
+constexpr uint32_t kNoPlace = 0xffffffffu;
+constexpr int64_t kNothing = -(int64_t(1) << 40);
 constexpr int kBiases = 512;              // entries of a chunk that are listed in shared memory
 
 template <typename T> struct Logit;
@@ -65,9 +67,10 @@ template <> struct Logit<float> {
   static __device__ __forceinline__ float largest(const uint4& v) {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
-  static __device__ __forceinline__ void mask(uint4& v, uint32_t bits) {
-    v.x = bits & 1u ? v.x : 0xff800000u; v.y = bits & 2u ? v.y : 0xff800000u;
-    v.z = bits & 4u ? v.z : 0xff800000u; v.w = bits & 8u ? v.w : 0xff800000u;
+  static constexpr uint32_t kLow = 0xff800000u, kNone = 0x7fffffffu;      // -inf, a NaN
+  static __device__ __forceinline__ void mask(uint4& v, uint32_t bits, uint32_t other) {
+    v.x = bits & 1u ? v.x : other; v.y = bits & 2u ? v.y : other;
+    v.z = bits & 4u ? v.z : other; v.w = bits & 8u ? v.w : other;
   }
 };
 // fp16 and bf16: the 16-bit keys of the arg-max kernel, so that their words compare.
@@ -76,9 +79,15 @@ __device__ __forceinline__ uint32_t key16(uint32_t bits, uint32_t infinity) {
   if (bits == 0x8000u) return 0x8000u;
   return bits & 0x8000u ? ~bits & 0xffffu : bits | 0x8000u;
 }
-__device__ __forceinline__ uint32_t mask16(uint32_t pair, uint32_t bits, uint32_t infinity) {
-  const uint32_t keep = (bits & 1u ? 0xffffu : 0u) | (bits & 2u ? 0xffff0000u : 0u);
-  return (pair & keep) | (infinity & ~keep);
+// Eight 16-bit values, those whose bit is 0 replaced by `other`.
+__device__ __forceinline__ void mask16(uint4& v, uint32_t bits, uint32_t other) {
+  // four bits to four bytes of ones or zeros (the factor puts bit i at bit 8i), each byte doubled
+  const uint32_t low = ((bits & 15u) * 0x204081u & 0x1010101u) * 255u, high = ((bits >> 4 & 15u) * 0x204081u & 0x1010101u) * 255u;
+  const uint32_t keep[4] = {__byte_perm(low, 0u, 0x1100), __byte_perm(low, 0u, 0x3322), __byte_perm(high, 0u, 0x1100), __byte_perm(high, 0u, 0x3322)};
+  v.x = (v.x & keep[0]) | (other & ~keep[0]);
+  v.y = (v.y & keep[1]) | (other & ~keep[1]);
+  v.z = (v.z & keep[2]) | (other & ~keep[2]);
+  v.w = (v.w & keep[3]) | (other & ~keep[3]);
 }
 template <> struct Logit<__half> {
   static constexpr int kVector = 8;
@@ -90,10 +99,8 @@ template <> struct Logit<__half> {
     const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
     return __hmax(__low2half(m), __high2half(m));
   }
-  static __device__ __forceinline__ void mask(uint4& v, uint32_t bits) {
-    v.x = mask16(v.x, bits, 0xfc00fc00u); v.y = mask16(v.y, bits >> 2, 0xfc00fc00u);
-    v.z = mask16(v.z, bits >> 4, 0xfc00fc00u); v.w = mask16(v.w, bits >> 6, 0xfc00fc00u);
-  }
+  static constexpr uint32_t kLow = 0xfc00fc00u, kNone = 0x7fff7fffu;
+  static __device__ __forceinline__ void mask(uint4& v, uint32_t bits, uint32_t other) { mask16(v, bits, other); }
 };
 template <> struct Logit<__nv_bfloat16> {
   static constexpr int kVector = 8;
@@ -105,10 +112,8 @@ template <> struct Logit<__nv_bfloat16> {
     const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
     return __hmax(__low2bfloat16(m), __high2bfloat16(m));
   }
-  static __device__ __forceinline__ void mask(uint4& v, uint32_t bits) {
-    v.x = mask16(v.x, bits, 0xff80ff80u); v.y = mask16(v.y, bits >> 2, 0xff80ff80u);
-    v.z = mask16(v.z, bits >> 4, 0xff80ff80u); v.w = mask16(v.w, bits >> 6, 0xff80ff80u);
-  }
+  static constexpr uint32_t kLow = 0xff80ff80u, kNone = 0x7fff7fffu;
+  static __device__ __forceinline__ void mask(uint4& v, uint32_t bits, uint32_t other) { mask16(v, bits, other); }
 };
 
 __device__ __forceinline__ unsigned long long word_of(uint32_t key, uint32_t token) {
@@ -122,11 +127,12 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // every CTA runs before another writes to it
   extern __shared__ __align__(16) uint32_t table_s[];   // with a history or biases: keys, counts, bit map, list of slots
-  uint32_t* count_s = table_s + kSlots;
-  uint32_t* marked_s = count_s + kSlots;
+  uint32_t* count_s = table_s + a.slots;
+  uint32_t* marked_s = count_s + a.slots;
   uint16_t* list_s = reinterpret_cast<uint16_t*>(marked_s + a.chunk / 32);
   __shared__ int bias_at_s[kBiases], bias_count_s[kLogitThreads / 32], listed_s;
   __shared__ float bias_s[kBiases];
+  __shared__ uint16_t bias_slot_s[kBiases];
   __shared__ unsigned long long part_s[kLogitThreads / 32], slice_s[kRanks];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   uint32_t rank, ranks;
@@ -148,24 +154,29 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
   const uint32_t* mask = reinterpret_cast<const uint32_t*>(a.mask) + m * a.mask_stride;
   const bool tracked = length > 0 || a.biases > 0;
 
-  const int begin = max(int(rank) * a.slice, shift), end = min(int(rank + 1) * a.slice, a.width + shift);
+  // the row's blocks of a piece for each thread go to the CTAs in turn, so that common tokens, which lie together, do not
+  // meet in one; a CTA numbers its own places through
+  constexpr int kBlock = kLogitThreads * V;
+  const int end = a.width + shift, turn = __ffs(ranks) - 1;
+  auto place_of = [&](int local) { return ((local / kBlock << turn) + int(rank)) * kBlock + local % kBlock; };
   unsigned long long top = 0;                  // of what the list takes
-  uint32_t key = 0, token = 0;                 // of the rest, which it meets in rising order
-  bool any = false;
+  uint32_t key = 0;                            // of the rest, which it meets in rising order: the largest key,
+  uint4 best{};                                // the first piece that has it, and that piece's token
+  int64_t token = kNothing;
   auto history = [&](int i) -> int64_t {
     return a.long_tokens ? __ldg(static_cast<const long long*>(a.tokens) + m * a.tokens_stride + i)
                          : __ldg(static_cast<const int*>(a.tokens) + m * a.tokens_stride + i);
   };
-  for (int base = int(rank) * a.slice;; base += a.chunk) {
-    const int low = max(base, begin), high = min(base + a.chunk, end);
-    const int64_t first = token0 + base;      // token of the chunk's first place
+  for (int base = 0;; base += a.chunk) {
+    const int last = min(base + a.chunk, a.slice);
     // the chunk's first logits, and their bits of the mask
     uint4 held[kDeep];
     uint64_t bits[kDeep];
-    const int place0 = base + int(threadIdx.x) * V;
-    auto load = [&](int i, int place) {
-      if (place >= high) return;
-      if (vectors && place >= low && place + V <= high) held[i] = *reinterpret_cast<const uint4*>(row + place);
+    const int first = base + int(threadIdx.x) * V;
+    auto load = [&](int i, int local) {
+      const int place = place_of(local);
+      if (local >= last || place >= end) return;
+      if (vectors && place >= shift && place + V <= end) held[i] = *reinterpret_cast<const uint4*>(row + place);
       if (a.mask) {
         const int64_t at = max(token0 + place, int64_t(0)), word = at >> 5;     // a place before the row's first token has no bit
         bits[i] = mask[word];
@@ -173,17 +184,24 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
       }
     };
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) load(i, place0 + i * kLogitThreads * V);
+    for (int i = 0; i < kDeep; ++i) load(i, first + i * kBlock);
+    // the number in the chunk of a token, or none
+    auto number = [&](int64_t id) {
+      const int64_t place = id - token0;
+      if (place < shift || place >= end) return kNoPlace;
+      const uint32_t block = uint32_t(place) / kBlock;
+      if ((block & (ranks - 1)) != rank) return kNoPlace;
+      const uint32_t at = (block >> turn) * kBlock + uint32_t(place) % kBlock - uint32_t(base);
+      return at < uint32_t(last - base) ? at : kNoPlace;
+    };
     // counts `add` for, or flags, the token at a place of the chunk
     auto note = [&](uint32_t at, uint32_t add, uint32_t flag) {
-      uint32_t slot = (at + 1) * 2654435761u >> 19;
-      static_assert(kSlots == 1 << 13, "the hash leaves 13 bits");
-      for (;; slot = (slot + 1) % kSlots) {
+      uint32_t slot = (at + 1) * 2654435761u >> (__clz(a.slots) + 1);
+      for (;; slot = (slot + 1) & (a.slots - 1)) {
         uint32_t key_there = *static_cast<volatile uint32_t*>(table_s + slot);
         if (key_there == 0) {
           key_there = atomicCAS(table_s + slot, 0u, at + 1);
           if (key_there == 0) {
-            list_s[atomicAdd(&listed_s, 1)] = uint16_t(slot);
             atomicOr(marked_s + at / 32, 1u << (at % 32));
             break;
           }
@@ -192,15 +210,15 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
       }
       if (flag) atomicOr(count_s + slot, flag);
       else atomicAdd(count_s + slot, add);
+      return slot;
     };
     if (tracked) {
-      for (int i = threadIdx.x * 4; i < 2 * kSlots + a.chunk / 32; i += kLogitThreads * 4) *reinterpret_cast<uint4*>(table_s + i) = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = threadIdx.x * 4; i < 2 * a.slots + a.chunk / 32; i += kLogitThreads * 4) *reinterpret_cast<uint4*>(table_s + i) = make_uint4(0u, 0u, 0u, 0u);
       if (threadIdx.x == 0) listed_s = 0;
       __syncthreads();
-      const int64_t from = first + (low - base);
-      const uint32_t size = uint32_t(high - low);
       auto count = [&](int i, int64_t id) {
-        if (uint64_t(id - from) < size) note(uint32_t(id - first), 1u, i >= prompt ? 0u : kSeen);
+        const uint32_t at = number(id);
+        if (at != kNoPlace) note(at, 1u, i >= prompt ? 0u : kSeen);
       };
       int i = threadIdx.x;
       for (; i + 3 * kLogitThreads < length; i += 4 * kLogitThreads) {
@@ -216,8 +234,8 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
     int biases = 0;
     for (int group = 0; group < a.biases; group += kLogitThreads) {
       const int entry = group + threadIdx.x;
-      const int64_t id = entry < a.biases ? a.bias_tokens[m * a.bias_stride + entry] : -1, at = id - first;
-      const bool inside = id >= 0 && at >= low - base && at < high - base;
+      const uint32_t at = entry < a.biases ? number(a.bias_tokens[m * a.bias_stride + entry]) : kNoPlace;
+      const bool inside = at != kNoPlace;
       const uint32_t votes = __ballot_sync(0xffffffffu, inside);
       if ((threadIdx.x & 31) == 0) bias_count_s[threadIdx.x >> 5] = __popc(votes);
       __syncthreads();
@@ -228,8 +246,9 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
         biases += bias_count_s[w];
       }
       if (inside) {
-        note(uint32_t(at), 0u, kBiased);
+        const uint32_t there = note(at, 0u, kBiased);
         if (slot < kBiases) {
+          bias_slot_s[slot] = uint16_t(there);
           bias_at_s[slot] = int(at);
           bias_s[slot] = a.bias[m * a.bias_stride + entry];
         }
@@ -237,79 +256,115 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
       __syncthreads();
     }
     if (tracked) __syncthreads();
-    for (int start = place0; start < high; start += kDeep * kLogitThreads * V) {
+    for (int start = first; start < last; start += kDeep * kBlock) {
 #pragma unroll
       for (int i = 0; i < kDeep; ++i) {
-        const int place = start + i * kLogitThreads * V, local = place - base;
-        if (place >= high) break;
+        const int local = start + i * kBlock, place = place_of(local);
+        if (local >= last || place >= end) break;
         const int64_t id = token0 + place;
-        if (!any) token = uint32_t(token0 + max(place, low));     // a row of NaN gives its first token
-        any = true;
-        const bool whole = place >= low && place + V <= high;
-        uint4 v = held[i];
-        T* values = reinterpret_cast<T*>(&v);
-        if (!(vectors && whole)) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) values[e] = place + e >= low && place + e < high ? row[place + e] : L::narrow(-INFINITY);
-        }
+        const uint32_t marked = tracked ? marked_s[(local - base) / 32] >> (local % 32) & ((1u << V) - 1) : 0u;
+        uint32_t allowed = ~0u;
         if (a.mask) {
           const int64_t at = max(id, int64_t(0));
-          L::mask(v, uint32_t(bits[i] >> (at & 31)) << (at - id));
+          allowed = uint32_t(bits[i] >> (at & 31)) << (at - id) | marked;
         }
-        load(i, place + kDeep * kLogitThreads * V);
-        const uint32_t marked = tracked ? marked_s[local / 32] >> (local % 32) & ((1u << V) - 1) : 0u;
-        if (vectors && whole && marked == 0) {
-          *reinterpret_cast<uint4*>(out + place) = v;
+        uint4 v = held[i];
+        const bool whole = vectors && place >= shift && place + V <= end;
+        if (whole) {
+          load(i, local + kDeep * kBlock);
+          if (a.mask) L::mask(v, allowed, L::kLow);
+          *reinterpret_cast<uint4*>(out + place) = v;      // marked tokens as they were: the list reads them, here or in `row`
         } else {
+          T* values = reinterpret_cast<T*>(&v);
+          uint32_t inside = 0;
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            if (place + e >= low && place + e < high && !(marked >> e & 1u)) out[place + e] = values[e];
-            else values[e] = L::narrow(__int_as_float(0x7fffffff));      // none, or one of the list
-          }
+          for (int e = 0; e < V; ++e) inside |= uint32_t(place + e >= shift && place + e < end) << e;
+#pragma unroll
+          for (int e = 0; e < V; ++e) values[e] = inside >> e & 1u ? row[place + e] : L::narrow(0.f);
+          load(i, local + kDeep * kBlock);
+          if (a.mask) L::mask(v, allowed, L::kLow);
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (inside >> e & 1u) out[place + e] = values[e];
+          L::mask(v, inside, L::kNone);
         }
+        if (marked) L::mask(v, ~marked, L::kNone);
         const uint32_t largest = L::key(L::largest(v));
-        if (largest > key) {
+        if (largest > key || token == kNothing) {
           key = largest;
-#pragma unroll
-          for (int e = V - 1; e >= 0; --e)
-            if (L::key(values[e]) == largest) token = uint32_t(id + e);
+          best = v;
+          token = id;
         }
       }
     }
     if (tracked) {
+      // the slots in use, listed warp by warp (a shared counter for each new token queued them all)
+      int used = 0;
+      for (int i = threadIdx.x; i < a.slots; i += kLogitThreads) used += table_s[i] != 0;
+      int before = used;
+#pragma unroll
+      for (int step = 1; step < 32; step <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, before, step);
+        if (int(threadIdx.x & 31) >= step) before += other;
+      }
+      int to = 0;
+      if ((threadIdx.x & 31) == 31) to = atomicAdd(&listed_s, before);
+      to = __shfl_sync(0xffffffffu, to, 31) + before - used;
+      for (int i = threadIdx.x; i < a.slots; i += kLogitThreads)
+        if (table_s[i] != 0) list_s[to++] = uint16_t(i);
       __syncthreads();
       const int listed = listed_s;
-      for (int i = threadIdx.x; i < listed; i += kLogitThreads) {
-        const int at = int(table_s[list_s[i]]) - 1;
-        const uint32_t count = count_s[list_s[i]];
-        const int64_t id = first + at;
-        float x = L::widen(row[base + at]);
+      auto finish = [&](int at, uint32_t count, float bias) {
+        const int place = place_of(base + at);
+        const int64_t id = token0 + place;
+        float x = L::widen(row[place]);
         if (count & (kSeen | kCount)) {
           x = x > 0.f ? __fdiv_rn(x, repetition) : __fmul_rn(x, repetition);
           x = __fsub_rn(x, __fmul_rn(frequency, float(count & kCount)));
           if (count & kCount) x = __fsub_rn(x, presence);
         }
-        if (count & kBiased) {      // added up in the order of the entries, in 64 bits
-          double sum = 0.0;
-          if (biases <= kBiases) {
-            for (int e = 0; e < biases; ++e) sum += bias_at_s[e] == at ? double(bias_s[e]) : 0.0;
-          } else {
-            for (int e = 0; e < a.biases; ++e) sum += a.bias_tokens[m * a.bias_stride + e] == id ? double(a.bias[m * a.bias_stride + e]) : 0.0;
-          }
-          x = __fadd_rn(x, float(sum));
-        }
+        if (count & kBiased) x = __fadd_rn(x, bias);
         if (a.mask && !(mask[id >> 5] >> (id & 31) & 1u)) x = -INFINITY;
         const T result = L::narrow(x);
-        out[base + at] = result;
+        out[place] = result;
         const unsigned long long word = word_of(L::key(result), uint32_t(id));
         top = word > top ? word : top;
+      };
+      // the biases of a token are added up in the order of the entries, in 64 bits
+      for (int i = threadIdx.x; i < listed; i += kLogitThreads) {
+        const int at = int(table_s[list_s[i]]) - 1;
+        const uint32_t count = count_s[list_s[i]];
+        double sum = 0.0;
+        if (count & kBiased) {
+          if (biases <= kBiases) continue;      // by the thread of its first entry, below
+          for (int e = 0; e < a.biases; ++e)
+            if (number(a.bias_tokens[m * a.bias_stride + e]) == uint32_t(at)) sum += a.bias[m * a.bias_stride + e];
+        }
+        finish(at, count, float(sum));
+      }
+      for (int i = threadIdx.x; i < biases && biases <= kBiases; i += kLogitThreads) {
+        const int at = bias_at_s[i];
+        double sum = 0.0;
+        bool first_entry = true;
+        for (int e = 0; e < biases; ++e) {
+          if (bias_at_s[e] != at) continue;
+          first_entry = first_entry && e >= i;
+          sum += bias_s[e];
+        }
+        if (first_entry) finish(at, count_s[bias_slot_s[i]], float(sum));
       }
     }
-    if (base + a.chunk >= end) break;
+    if (last == a.slice) break;
     __syncthreads();
   }
-  if (any) {
-    const unsigned long long word = word_of(key, token);
+  if (token != kNothing) {
+    const T* values = reinterpret_cast<const T*>(&best);
+    int first = V - 1;
+#pragma unroll
+    for (int e = V - 1; e >= 0; --e)
+      if (L::key(values[e]) == key) first = e;
+    // (nothing but NaN, and what is no token, in a piece: its first token)
+    const unsigned long long word = word_of(key, uint32_t(max(token + first, a.offset)));
     top = word > top ? word : top;
   }
 #pragma unroll
@@ -343,14 +398,12 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
   }
 }
 
-constexpr int kTableBytes = kSlots * 8 + kMost * 2;
-
 template <typename T>
 int launch_logits(const LogitArguments& a, int M, int ranks, void* stream) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(ranks, M);
   config.blockDim = dim3(kLogitThreads);
-  config.dynamicSmemBytes = a.tokens || a.bias ? kTableBytes + a.chunk / 8 : 0;
+  config.dynamicSmemBytes = a.tokens || a.bias ? a.slots * 8 + a.slots * 3 / 4 * 2 + a.chunk / 8 : 0;
   int device = 0;
   cudaGetDevice(&device);
   static std::atomic<uint64_t> opted{0};
@@ -398,13 +451,20 @@ extern "C" int mkb_adjust_logits(const void* logits, void* out, const void* toke
               (long long)mask_words, (long long)(offset + width));
   LogitArguments a{logits, out, history ? tokens : nullptr, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, mask,
                    static_cast<unsigned long long*>(best), static_cast<long long*>(picked), logits_stride, out_stride, tokens_stride,
-                   bias_stride, mask_words, mask_stride, offset, int(width), int(history), bias ? int(biases) : 0, long_tokens, 0, 0};
+                   bias_stride, mask_words, mask_stride, offset, int(width), int(history), bias ? int(biases) : 0, long_tokens, 0, 0, 0};
   // CTAs of a row: up to sixteen, of 4096 tokens or more (one piece a thread), and two an SM in all
   int ranks = 1;
   while (ranks < kRanks && int64_t(ranks) * 4096 < width && int64_t(ranks) * M <= device_info().sm_count) ranks *= 2;
-  a.slice = int((width + 7 + ranks - 1) / ranks + 127) / 128 * 128;
-  // a chunk holds no more tokens of a history than the table takes, and its bit map is 64 KB at most
-  a.chunk = (a.tokens ? history : 0) + a.biases <= kMost ? (a.slice < 1 << 19 ? a.slice : 1 << 19) : kMost;
+  // a CTA's places: as many blocks of a piece for each thread as the longest of them has; a chunk has no more tokens than the
+  // table takes, unless history and biases together have no more, and then a bit map of 64 KB at most
+  const int block = kLogitThreads * (dtype == MKB_F32 ? 4 : 8), blocks = int((width + 7 + block - 1) / block);
+  a.slice = (blocks + ranks - 1) / ranks * block;
+  const int64_t noted = (a.tokens ? history : 0) + a.biases;
+  a.chunk = noted <= kMost ? (a.slice < 1 << 19 ? a.slice : 1 << 19) : block;
+  a.slots = kLogitThreads;
+  while (a.slots < kSlots && a.slots * 3 / 4 < noted) a.slots *= 2;
+  static_assert(kMost == kSlots * 3 / 4, "the table's size");
+  static_assert(kLogitThreads * 8 <= kMost, "a block fits the table");
   switch (dtype) {
     case MKB_F16: return launch_logits<__half>(a, M, ranks, stream);
     case MKB_BF16: return launch_logits<__nv_bfloat16>(a, M, ranks, stream);
