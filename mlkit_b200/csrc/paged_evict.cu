@@ -2,6 +2,8 @@
 // min(n, budget): the first `sinks`, the last `recent`, and of the others the heaviest, a tie going to the lower slot.  The
 // kept slots, in their order, move to fresh pages with their keys, values and weights, so a page that other sequences read
 // as well stays as it is, and no move waits for another.
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace mkb {
@@ -19,18 +21,22 @@ __device__ __forceinline__ uint32_t key_of(float weight) {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kHeldKeys = 49152;      // keys of a sequence that lie in shared memory; longer ones are read again for each digit
 
 // One CTA per (head, sequence).  The border between kept and dropped weights is found digit by digit, most significant
-// first: a histogram of the candidates that share the digits found so far says in which bin the last kept weight lies.
-// Then every warp lists what it keeps of its own run of slots.
+// first: a histogram of the candidates that share the digits found so far says in which bin the last kept weight lies.  A
+// warp's equal digits are counted by one of its lanes: many slots have the same small weight, or one of a few exponents, and
+// queued at their bin.  Then every warp lists what it keeps of its own run of slots.  What bounds it is the chain of four
+// digits for a CTA of 16 keys a thread; the moves that follow take most of the time.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedLayout layout, const float* __restrict__ weights,
                                                                       const int* __restrict__ lengths, int* __restrict__ kept,
-                                                                      int kv_heads, int budget, int sinks, int recent) {
+                                                                      int kv_heads, int budget, int sinks, int recent, int held) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  extern __shared__ uint32_t key_s[];      // [held]
   __shared__ uint32_t bins_s[256];
   __shared__ uint32_t count_s[kSelectWarps][2];
-  __shared__ uint32_t found_s[2];
+  __shared__ uint32_t found_s[3];
   const int head = blockIdx.x, m = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int* table = layout.tables + m * layout.table_stride;
   int* list = kept + (int64_t(m) * kv_heads + head) * budget;
@@ -46,57 +52,88 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedLayou
   }
   const int low = sinks, high = n - recent;          // candidates: [low, high)
   int want = budget - sinks - recent;                // of which this many stay
-  auto key_at = [&](int p) {
+  auto read_key = [&](int p) {
     const int64_t at = layout.weight_of(table, kv_heads, head, p);
     if (at < 0) {
       atomicOr(&g_paged_evict_status, 1u);
       return 0u;
     }
-    return key_of(weights[at]);
+    return key_of(__ldg(weights + at));
   };
-  uint32_t prefix = 0;
-#pragma unroll 1
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kSelectThreads) bins_s[i] = 0;
-    __syncthreads();
-    for (int p = low + threadIdx.x; p < high; p += kSelectThreads) {
-      const uint32_t key = key_at(p);
-      if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&bins_s[(key >> shift) & 255u], 1u);
+  const bool all_held = high <= held;
+  if (all_held) {
+    int p = low + threadIdx.x;
+    for (; p + 3 * kSelectThreads < high; p += 4 * kSelectThreads) {
+      uint32_t keys[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) keys[u] = read_key(p + u * kSelectThreads);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) key_s[p + u * kSelectThreads] = keys[u];
     }
-    __syncthreads();
-    if (warp == 0) {   // lane l holds bins 255 - 8l down to 248 - 8l: a scan from the heaviest bin
-      uint32_t own = 0, bin[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) own += bin[i] = bins_s[255 - 8 * lane - i];
-      uint32_t before = own;
-#pragma unroll
-      for (int step = 1; step < 32; step <<= 1) {
-        const uint32_t other = __shfl_up_sync(0xffffffffu, before, step);
-        if (lane >= step) before += other;
-      }
-      before -= own;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (before < uint32_t(want) && before + bin[i] >= uint32_t(want)) { found_s[0] = 255 - 8 * lane - i; found_s[1] = before; }
-        before += bin[i];
-      }
-      if (want == 0 && lane == 0) { found_s[0] = 255; found_s[1] = 0; }
-    }
-    __syncthreads();
-    prefix = prefix << 8 | found_s[0];
-    want -= int(found_s[1]);
-    __syncthreads();
+    for (; p < high; p += kSelectThreads) key_s[p] = read_key(p);
   }
-  // prefix: the lightest weight kept; `want`: how many of those that equal it stay (none when nothing but the safe slots does)
+  auto key_at = [&](int p) { return all_held ? key_s[p] : read_key(p); };
+  // keys over `edge` stay, and of those that equal it the first `want`
+  uint32_t edge = 0xffffffffu;
+  if (want == 0) {
+    __syncthreads();
+  } else {
+    uint32_t prefix = 0;
+#pragma unroll 1
+    for (int shift = 24;; shift -= 8) {
+      if (threadIdx.x < 256) bins_s[threadIdx.x] = 0;
+      __syncthreads();
+      for (int p = low + threadIdx.x; p - lane < high; p += kSelectThreads) {
+        const uint32_t key = p < high ? key_at(p) : 0u;
+        const bool counts = p < high && (shift == 24 || (key >> (shift + 8)) == prefix);
+        const uint32_t digit = counts ? (key >> shift) & 255u : 256u;
+        const uint32_t same = __match_any_sync(0xffffffffu, digit);
+        if (counts && lane == __ffs(same) - 1) atomicAdd(&bins_s[digit], __popc(same));
+      }
+      __syncthreads();
+      if (warp == 0) {   // lane l holds bins 255 - 8l down to 248 - 8l: a scan from the heaviest bin
+        uint32_t own = 0, bin[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) own += bin[i] = bins_s[255 - 8 * lane - i];
+        uint32_t before = own;
+#pragma unroll
+        for (int step = 1; step < 32; step <<= 1) {
+          const uint32_t other = __shfl_up_sync(0xffffffffu, before, step);
+          if (lane >= step) before += other;
+        }
+        before -= own;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (before < uint32_t(want) && before + bin[i] >= uint32_t(want)) { found_s[0] = 255 - 8 * lane - i; found_s[1] = before; found_s[2] = bin[i]; }
+          before += bin[i];
+        }
+      }
+      __syncthreads();
+      prefix = prefix << 8 | found_s[0];
+      want -= int(found_s[1]);
+      const bool whole_bin = found_s[2] == uint32_t(want);
+      if (shift == 0) {
+        edge = prefix;
+        break;
+      }
+      if (whole_bin) {      // everything with these digits stays: no key is lower than the one before them
+        edge = (prefix << shift) - 1;
+        want = 0;
+        break;
+      }
+      __syncthreads();
+    }
+  }
   const int run = (n + kSelectThreads - 1) / kSelectThreads * 32;
   const int first = warp * run, last = min(first + run, n);
+  const bool chosen = budget > sinks + recent;
   auto sort_out = [&](int p, bool& over, bool& level) {
     over = level = false;
     if (p >= last) return;
     if (p < low || p >= high) { over = true; return; }
     const uint32_t key = key_at(p);
-    over = key > prefix && budget > sinks + recent;
-    level = key == prefix;
+    over = chosen && key > edge;
+    level = key == edge;
   };
   uint32_t overs = 0, levels = 0;
   bool over, level;
@@ -121,29 +158,53 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedLayou
 }
 
 constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 4;      // rows of a thread under way
 
-// A thread moves one 16-byte vector of a key and of a value.
+// A thread moves 16-byte vectors of keys and of values, of kMoveRows rows at a time.  Bound by memory: 4 * head_dim bytes
+// read and as many written for a row.
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(PagedLayout from, PagedLayout to, uint4* __restrict__ k_pages,
                                                                   uint4* __restrict__ v_pages, float* __restrict__ weights,
                                                                   const int* __restrict__ kept, int kv_heads, int budget, int vectors) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int head = blockIdx.y, m = blockIdx.z;
-  const uint32_t index = blockIdx.x * kMoveThreads + threadIdx.x;
-  const uint32_t row = index / vectors, vector = index - row * vectors;
-  if (row >= uint32_t(budget)) return;
-  const int old = kept[(int64_t(m) * kv_heads + head) * budget + row];
-  if (old < 0) return;
+  const int rows = kMoveThreads / vectors;      // of a pass of the block
+  const int own = threadIdx.x / vectors, vector = threadIdx.x - own * vectors;
+  if (own >= rows) return;
+  const int row0 = blockIdx.x * rows * kMoveRows + own;
+  const int* list = kept + (int64_t(m) * kv_heads + head) * budget;
   const int* old_table = from.tables + m * from.table_stride;
   const int* new_table = to.tables + m * to.table_stride;
-  const uint32_t source = from.vector_of(old_table, head, old), target = to.vector_of(new_table, head, row);
-  if (source == kNoSlot || target == kNoSlot) {
-    atomicOr(&g_paged_evict_status, 1u);
-    return;
+  int old[kMoveRows];
+#pragma unroll
+  for (int i = 0; i < kMoveRows; ++i) old[i] = row0 + i * rows < budget ? __ldg(list + row0 + i * rows) : -1;
+  uint32_t source[kMoveRows], target[kMoveRows];
+#pragma unroll
+  for (int i = 0; i < kMoveRows; ++i) {
+    source[i] = target[i] = kNoSlot;
+    if (old[i] < 0) continue;
+    source[i] = from.vector_of(old_table, head, old[i]);
+    target[i] = to.vector_of(new_table, head, row0 + i * rows);
+    if (source[i] == kNoSlot || target[i] == kNoSlot) {
+      atomicOr(&g_paged_evict_status, 1u);
+      source[i] = kNoSlot;
+    }
   }
-  k_pages[int64_t(target) + vector] = k_pages[int64_t(source) + vector];
-  v_pages[int64_t(target) + vector] = v_pages[int64_t(source) + vector];
-  if (vector == 0) weights[to.weight_of(new_table, kv_heads, head, row)] = weights[from.weight_of(old_table, kv_heads, head, old)];
+  uint4 key[kMoveRows], value[kMoveRows];
+#pragma unroll
+  for (int i = 0; i < kMoveRows; ++i)
+    if (source[i] != kNoSlot) {
+      key[i] = k_pages[int64_t(source[i]) + vector];
+      value[i] = v_pages[int64_t(source[i]) + vector];
+    }
+#pragma unroll
+  for (int i = 0; i < kMoveRows; ++i)
+    if (source[i] != kNoSlot) {
+      k_pages[int64_t(target[i]) + vector] = key[i];
+      v_pages[int64_t(target[i]) + vector] = value[i];
+      if (vector == 0)
+        weights[to.weight_of(new_table, kv_heads, head, row0 + i * rows)] = weights[from.weight_of(old_table, kv_heads, head, old[i])];
+    }
 }
 
 }  // namespace
@@ -177,14 +238,23 @@ extern "C" int mkb_paged_evict(void* k_pages, void* v_pages, float* weights, con
   if (status != MKB_OK) return status;
   MKB_REQUIRE(int64_t(new_columns) * page >= budget || int64_t(new_columns) * page >= int64_t(columns) * page, MKB_E_ARGUMENT,
               "%s: %d new pages of %d slots do not hold the budget of %d", what, new_columns, page, budget);
-  cudaError_t launched = launch_dependent(evict_select_kernel, dim3(kv_heads, M), dim3(kSelectThreads), 0, stream, from,
-                                          static_cast<const float*>(weights), lengths, kept, kv_heads, budget, sinks, recent);
+  const int64_t capacity = int64_t(columns) * page;
+  const int held = capacity < kHeldKeys ? int(capacity) : kHeldKeys;
+  int device = 0;
+  cudaGetDevice(&device);
+  static std::atomic<uint64_t> opted{0};
+  if (!(opted.load(std::memory_order_acquire) >> (device & 63) & 1)) {
+    const cudaError_t set = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldKeys * 4);
+    if (set != cudaSuccess) return cuda_fail(set, "paged evict shared memory");
+    opted.fetch_or(uint64_t(1) << (device & 63), std::memory_order_release);
+  }
+  cudaError_t launched = launch_dependent(evict_select_kernel, dim3(kv_heads, M), dim3(kSelectThreads), size_t(held) * 4, stream, from,
+                                          static_cast<const float*>(weights), lengths, kept, kv_heads, budget, sinks, recent, held);
   if (launched != cudaSuccess) return cuda_fail(launched, "paged evict launch");
-  const int vectors = head_dim / 8;
-  const int64_t blocks = (int64_t(budget) * vectors + kMoveThreads - 1) / kMoveThreads;
-  launched = launch_dependent(evict_move_kernel, dim3(unsigned(blocks), kv_heads, M), dim3(kMoveThreads), 0, stream, from, to,
-                              static_cast<uint4*>(k_pages), static_cast<uint4*>(v_pages), weights, static_cast<const int*>(kept),
-                              kv_heads, budget, vectors);
+  const int vectors = head_dim / 8, rows = kMoveThreads / vectors * kMoveRows;
+  launched = launch_dependent(evict_move_kernel, dim3(unsigned((int64_t(budget) + rows - 1) / rows), kv_heads, M), dim3(kMoveThreads), 0, stream,
+                              from, to, static_cast<uint4*>(k_pages), static_cast<uint4*>(v_pages), weights,
+                              static_cast<const int*>(kept), kv_heads, budget, vectors);
   if (launched != cudaSuccess) return cuda_fail(launched, "paged evict launch");
   return MKB_OK;
 }
