@@ -27,7 +27,8 @@ constexpr int kHeldKeys = 49152;      // keys of a sequence that lie in shared m
 // first: a histogram of the candidates that share the digits found so far says in which bin the last kept weight lies.  A
 // warp's equal digits are counted by one of its lanes: many slots have the same small weight, or one of a few exponents, and
 // queued at their bin.  Then every warp lists what it keeps of its own run of slots.  What bounds it is the chain of four
-// digits for a CTA of 16 keys a thread; the moves that follow take most of the time.
+// digits for a CTA of 16 keys a thread, 30 of the 114 us for 16 x 8 sequences of up to 16384 slots; digits of 12 and 10 bits
+// with the counts queueing, or with only the most common digit of a warp counted by a vote, measured no better.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedLayout layout, const float* __restrict__ weights,
                                                                       const int* __restrict__ lengths, int* __restrict__ kept,
                                                                       int kv_heads, int budget, int sinks, int recent, int held) {
@@ -158,53 +159,61 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedLayou
 }
 
 constexpr int kMoveThreads = 256;
-constexpr int kMoveRows = 4;      // rows of a thread under way
+constexpr int kMoveRows = 64;     // of a block
+constexpr int kMoveDeep = 4;      // vectors of keys, and of values, of a thread under way
 
-// A thread moves 16-byte vectors of keys and of values, of kMoveRows rows at a time.  Bound by memory: 4 * head_dim bytes
-// read and as many written for a row.
+// A block looks up where its rows come from and go to, a thread for each, moving their weights; then its threads move the
+// rows' 16-byte vectors.  (The look-up by each thread for its own vectors made every copy wait for three loads in turn: 110
+// us for 16 x 8 x 4096 rows of 256 bytes, against 78 at the copy rate.)  Bound by memory: 4 * head_dim bytes read and as many written
+// for a row, which are not read again soon, so they pass the caches as streams.
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(PagedLayout from, PagedLayout to, uint4* __restrict__ k_pages,
                                                                   uint4* __restrict__ v_pages, float* __restrict__ weights,
                                                                   const int* __restrict__ kept, int kv_heads, int budget, int vectors) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int head = blockIdx.y, m = blockIdx.z;
-  const int rows = kMoveThreads / vectors;      // of a pass of the block
-  const int own = threadIdx.x / vectors, vector = threadIdx.x - own * vectors;
-  if (own >= rows) return;
-  const int row0 = blockIdx.x * rows * kMoveRows + own;
-  const int* list = kept + (int64_t(m) * kv_heads + head) * budget;
-  const int* old_table = from.tables + m * from.table_stride;
-  const int* new_table = to.tables + m * to.table_stride;
-  int old[kMoveRows];
-#pragma unroll
-  for (int i = 0; i < kMoveRows; ++i) old[i] = row0 + i * rows < budget ? __ldg(list + row0 + i * rows) : -1;
-  uint32_t source[kMoveRows], target[kMoveRows];
-#pragma unroll
-  for (int i = 0; i < kMoveRows; ++i) {
-    source[i] = target[i] = kNoSlot;
-    if (old[i] < 0) continue;
-    source[i] = from.vector_of(old_table, head, old[i]);
-    target[i] = to.vector_of(new_table, head, row0 + i * rows);
-    if (source[i] == kNoSlot || target[i] == kNoSlot) {
-      atomicOr(&g_paged_evict_status, 1u);
-      source[i] = kNoSlot;
+  __shared__ uint2 move_s[kMoveRows];     // source and target, in vectors
+  const int head = blockIdx.y, m = blockIdx.z, row0 = blockIdx.x * kMoveRows;
+  const int rows = min(kMoveRows, budget - row0);
+  if (int(threadIdx.x) < rows) {
+    const int row = row0 + threadIdx.x, old = __ldg(kept + (int64_t(m) * kv_heads + head) * budget + row);
+    uint2 move = make_uint2(kNoSlot, kNoSlot);
+    if (old >= 0) {
+      const int* old_table = from.tables + m * from.table_stride;
+      const int* new_table = to.tables + m * to.table_stride;
+      move = make_uint2(from.vector_of(old_table, head, old), to.vector_of(new_table, head, row));
+      if (move.x == kNoSlot || move.y == kNoSlot) {
+        atomicOr(&g_paged_evict_status, 1u);
+        move.x = kNoSlot;
+      } else {
+        weights[to.weight_of(new_table, kv_heads, head, row)] = weights[from.weight_of(old_table, kv_heads, head, old)];
+      }
     }
+    move_s[threadIdx.x] = move;
   }
-  uint4 key[kMoveRows], value[kMoveRows];
+  __syncthreads();
+  const int total = rows * vectors;
+  for (int start = threadIdx.x; start < total; start += kMoveDeep * kMoveThreads) {
+    uint4 key[kMoveDeep], value[kMoveDeep];
+    int64_t target[kMoveDeep];
 #pragma unroll
-  for (int i = 0; i < kMoveRows; ++i)
-    if (source[i] != kNoSlot) {
-      key[i] = k_pages[int64_t(source[i]) + vector];
-      value[i] = v_pages[int64_t(source[i]) + vector];
+    for (int i = 0; i < kMoveDeep; ++i) {
+      const int index = start + i * kMoveThreads, row = index / vectors;
+      target[i] = -1;
+      if (index >= total) continue;
+      const uint2 move = move_s[row];
+      if (move.x == kNoSlot) continue;
+      const int vector = index - row * vectors;
+      key[i] = __ldcs(k_pages + (int64_t(move.x) + vector));
+      value[i] = __ldcs(v_pages + (int64_t(move.x) + vector));
+      target[i] = int64_t(move.y) + vector;
     }
 #pragma unroll
-  for (int i = 0; i < kMoveRows; ++i)
-    if (source[i] != kNoSlot) {
-      k_pages[int64_t(target[i]) + vector] = key[i];
-      v_pages[int64_t(target[i]) + vector] = value[i];
-      if (vector == 0)
-        weights[to.weight_of(new_table, kv_heads, head, row0 + i * rows)] = weights[from.weight_of(old_table, kv_heads, head, old[i])];
-    }
+    for (int i = 0; i < kMoveDeep; ++i)
+      if (target[i] >= 0) {
+        __stcs(k_pages + target[i], key[i]);
+        __stcs(v_pages + target[i], value[i]);
+      }
+  }
 }
 
 }  // namespace
@@ -251,10 +260,9 @@ extern "C" int mkb_paged_evict(void* k_pages, void* v_pages, float* weights, con
   cudaError_t launched = launch_dependent(evict_select_kernel, dim3(kv_heads, M), dim3(kSelectThreads), size_t(held) * 4, stream, from,
                                           static_cast<const float*>(weights), lengths, kept, kv_heads, budget, sinks, recent, held);
   if (launched != cudaSuccess) return cuda_fail(launched, "paged evict launch");
-  const int vectors = head_dim / 8, rows = kMoveThreads / vectors * kMoveRows;
-  launched = launch_dependent(evict_move_kernel, dim3(unsigned((int64_t(budget) + rows - 1) / rows), kv_heads, M), dim3(kMoveThreads), 0, stream,
+  launched = launch_dependent(evict_move_kernel, dim3(unsigned((int64_t(budget) + kMoveRows - 1) / kMoveRows), kv_heads, M), dim3(kMoveThreads), 0, stream,
                               from, to, static_cast<uint4*>(k_pages), static_cast<uint4*>(v_pages), weights,
-                              static_cast<const int*>(kept), kv_heads, budget, vectors);
+                              static_cast<const int*>(kept), kv_heads, budget, head_dim / 8);
   if (launched != cudaSuccess) return cuda_fail(launched, "paged evict launch");
   return MKB_OK;
 }
