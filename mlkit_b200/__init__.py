@@ -24,6 +24,7 @@ from mlkit_b200.inference import (
     packed_compatible,
 )
 from mlkit_b200.models import LayerReport, Model, QModel
+from mlkit_b200.paging import LogitRules, PagedCache
 from mlkit_b200.quantization import (
     Ctx,
     Grid,
@@ -48,7 +49,7 @@ from mlkit_b200.transforms import hadamard, randomized_transform, rht, structure
 __version__ = "0.1.0"
 
 __all__ = [
-    "BenchmarkResult", "Ctx", "Grid", "LayerReport", "Model", "PackedEmbedding", "PackedLayout", "PackedLinear",
+    "BenchmarkResult", "Ctx", "Grid", "LayerReport", "LogitRules", "Model", "PagedCache", "PackedEmbedding", "PackedLayout", "PackedLinear",
     "Q", "QModel", "Scaled", "as_q", "benchmark", "benchmark_model", "codec", "decode_feedback", "decode_scaled",
     "CapturedCall", "capture", "decoder", "fuse_siblings", "grid", "hadamard", "install_transform", "int", "layer_seed", "layout_for", "load",
     "load_checkpoint", "nf4", "optimize", "pack", "packed_compatible", "quantize", "randomized_transform",

@@ -11,13 +11,16 @@ block to ``transformers``); it is what serves the packed matvec on one 8-GPU box
   activations and the partial results are summed by one all-reduce per projection, two per layer;
 * between the matvecs: fused residual-add + RMS norm, rotary embedding + KV-cache append,
   single-token grouped-query attention, SiLU * up (``csrc/decode_ops.cu``);
-* a decode step for a fixed batch is captured once in a CUDA graph and replayed.
+* a decode step for a fixed batch is captured once in a CUDA graph and replayed;
+* with ``page`` given the keys and values lie in a ``PagedCache`` instead of a block of ``capacity`` slots per sequence, and the
+  attention is the one over pages; ``LogitRules`` adjust the logits before the pick.
 
 Sharding happens when the model is built; nothing sharded is ever written to a checkpoint.
 """
 
 import math
 import os
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -25,6 +28,7 @@ import torch.distributed as dist
 from torch import Tensor
 
 from mlkit_b200 import _native, kernels
+from mlkit_b200.paging import LogitRules, PagedCache
 from mlkit_b200.quantization import Q, pack
 
 
@@ -276,8 +280,13 @@ class TensorParallelDecoder:
     """One rank of a tensor-parallel Llama-shaped decoder with packed block linears."""
 
     def __init__(self, config: DecoderConfig, *, rank: int = 0, world: int = 1, device: torch.device | str = "cuda",
-                 max_batch: int = 8, capacity: int = 1024, group: "dist.ProcessGroup | None" = None) -> None:
+                 max_batch: int = 8, capacity: int = 1024, group: "dist.ProcessGroup | None" = None, page: int | None = None,
+                 pages: int | None = None, track_weights: bool = False) -> None:
+        """``page``: slots of a page of a ``PagedCache`` of ``pages`` pages (default: enough for ``max_batch`` sequences of
+        ``capacity`` slots), which with ``track_weights`` can evict.  Its rows begin with ``cache.open``."""
         config.validate(world)
+        if page is None and (pages is not None or track_weights):
+            raise ValueError("pages and tracked weights belong to a paged cache: give its page size")
         self.config, self.rank, self.world, self.group = config, rank, world, group
         self.device = torch.device(device)
         self.max_batch, self.capacity = max_batch, capacity
@@ -291,6 +300,9 @@ class TensorParallelDecoder:
         self.v_cache: list[Tensor] = []
         self._work: dict[int, dict[str, Tensor]] = {}
         self.exchange: PeerExchange | None = None
+        self.cache = None if page is None else PagedCache(
+            rows=max_batch, columns=-(-capacity // page), kv_heads=config.kv_heads // world, head_dim=config.head_dim, page=page,
+            pages=pages, device=self.device, track_weights=track_weights)
 
     def enable_peer_exchange(self) -> None:
         """Replace the library all-reduce after o and down by the one-shot peer-memory reduction."""
@@ -304,6 +316,9 @@ class TensorParallelDecoder:
         self.blocks.append(shards)
         self.norms.append((attention_norm.to(self.device).half().contiguous(),
                            mlp_norm.to(self.device).half().contiguous()))
+        if self.cache is not None:
+            self.cache.add_layer()
+            return
         shape = (self.max_batch, local_kv, self.capacity, config.head_dim)
         self.k_cache.append(torch.zeros(shape, dtype=torch.float16, device=self.device))
         self.v_cache.append(torch.zeros(shape, dtype=torch.float16, device=self.device))
@@ -344,6 +359,8 @@ class TensorParallelDecoder:
 
     def fill_cache(self, length: int, seed: int = 0) -> None:
         """A synthetic context: random keys and values for positions ``0..length-1`` of every sequence."""
+        if self.cache is not None:
+            raise ValueError("a paged cache is filled with cache.write")
         generator = torch.Generator(device=self.device).manual_seed(seed + 17 + self.rank)
         for cache in (*self.k_cache, *self.v_cache):
             cache[:, :, :length].copy_(torch.randn(cache[:, :, :length].shape, device=self.device,
@@ -380,16 +397,22 @@ class TensorParallelDecoder:
         if self.world > 1:
             dist.all_reduce(tensor, group=self.group)
 
-    def step(self, tokens: Tensor, positions: Tensor, greedy: bool = False) -> Tensor:
+    def step(self, tokens: Tensor, positions: Tensor, greedy: bool = False, rules: LogitRules | None = None) -> Tensor:
         """Decode one token per sequence: ``tokens`` int64 [batch], ``positions`` int32 [batch] (the
-        cache slot each new token takes).  Returns this step's logits [batch, vocab] in fp16, or, with
+        cache slot each new token takes; with a paged cache the token's position in the text alone, the slot being the
+        next of the row's sequence, and a row that is not in use gives logits of no meaning).  Returns this step's logits [batch, vocab] in fp16, or, with
         ``greedy``, the next tokens int64 [batch]: every rank picks the best token of its vocabulary
-        shard and the ranks exchange 8 bytes per sequence instead of their logits."""
+        shard and the ranks exchange 8 bytes per sequence instead of their logits.  ``rules`` adjust the logits of the first
+        ``batch`` rows, and with ``greedy`` observe the tokens picked."""
         c, w = self.config, self.world
         batch = tokens.shape[0]
         if batch > self.max_batch:
             raise ValueError(f"batch {batch} exceeds max_batch {self.max_batch}")
-        if not torch.cuda.is_current_stream_capturing():
+        cache, capturing = self.cache, torch.cuda.is_current_stream_capturing()
+        if cache is not None:
+            if not capturing:
+                cache.prepare(batch)
+        elif not capturing:
             # an eager step checks its cache slots on the host (one small synchronisation).  A captured
             # step cannot: its caller keeps positions below the capacity; the kernels clamp a position
             # that is not and report it through kernels.decode_status()
@@ -404,20 +427,24 @@ class TensorParallelDecoder:
         exchange = self.exchange
         for index, block in enumerate(self.blocks):
             attention_norm, mlp_norm = self.norms[index]
-            k_cache, v_cache = self.k_cache[index], self.v_cache[index]
             if exchange is not None and delta is not None:
                 exchange.reduce_add_rmsnorm(delta, residual, attention_norm, normed, c.eps)   # the down-projection shards
             else:
                 kernels.add_rmsnorm(residual, delta, attention_norm, normed, c.eps)
             block["qkv"](normed, work["qkv"])
-            if local_q <= 8 * local_kv and c.head_dim == 128:   # rotary embedding, cache append and attention in one launch
-                kernels.rope_attention_decode(work["qkv"], positions, k_cache, v_cache, work["attention"],
+            if cache is not None:
+                kernels.paged_rope_attention_decode(
+                    work["qkv"], positions, cache.lengths[:batch], cache.k_pages[index], cache.v_pages[index],
+                    cache.tables[:batch], work["attention"], q_heads=local_q, kv_heads=local_kv, head_dim=c.head_dim,
+                    theta=c.rope_theta, weights=cache.weights[index] if cache.track_weights else None)
+            elif local_q <= 8 * local_kv and c.head_dim == 128:   # rotary embedding, cache append and attention in one launch
+                kernels.rope_attention_decode(work["qkv"], positions, self.k_cache[index], self.v_cache[index], work["attention"],
                                               q_heads=local_q, kv_heads=local_kv, head_dim=c.head_dim,
                                               theta=c.rope_theta)
             else:
-                kernels.rope_append(work["qkv"], positions, k_cache, v_cache, q_heads=local_q, kv_heads=local_kv,
+                kernels.rope_append(work["qkv"], positions, self.k_cache[index], self.v_cache[index], q_heads=local_q, kv_heads=local_kv,
                                     head_dim=c.head_dim, theta=c.rope_theta)
-                kernels.attention_decode(work["qkv"], positions, k_cache, v_cache, work["attention"],
+                kernels.attention_decode(work["qkv"], positions, self.k_cache[index], self.v_cache[index], work["attention"],
                                          q_heads=local_q, kv_heads=local_kv, head_dim=c.head_dim)
             block["o"](work["attention"], work["o"])
             if exchange is not None:
@@ -441,41 +468,63 @@ class TensorParallelDecoder:
             self.packed_head(normed, work["logits"])
         else:
             torch.matmul(normed, self.head.t(), out=work["logits"])
+        if cache is not None:
+            cache.count(batch)
+            if not capturing:
+                cache.advance(batch)
+        share = work["logits"].shape[1]
+        if rules is not None:
+            rules.apply(work["logits"], offset=self.rank * share, best=work["keys"] if greedy else None)
         if greedy:
-            share = work["logits"].shape[1]
-            keys = kernels.argmax_keys(work["logits"], work["keys"], offset=self.rank * share)
+            keys = work["keys"]
+            if rules is None:
+                kernels.argmax_keys(work["logits"], keys, offset=self.rank * share)
             if w > 1:
                 dist.all_gather_into_tensor(work["all_keys"], keys, group=self.group)
                 keys = best_keys(work["all_keys"])
-            return kernels.tokens_of_keys(keys)
+            picked = kernels.tokens_of_keys(keys)
+            if rules is not None:
+                rules.observe(picked)
+            return picked
         if w == 1:
             return work["logits"]
         dist.all_gather_into_tensor(work["gathered"], work["logits"], group=self.group)
         return work["gathered"].permute(1, 0, 2).reshape(batch, c.vocab)
 
-    def capture(self, batch: int) -> "CapturedStep":
-        return CapturedStep(self, batch)
+    def capture(self, batch: int, greedy: bool = False, rules: LogitRules | None = None) -> "CapturedStep":
+        return CapturedStep(self, batch, greedy, rules)
 
 
 class CapturedStep:
-    """A decode step for a fixed batch as a CUDA graph: write ``tokens`` / ``positions``, ``replay()``."""
+    """A decode step for a fixed batch as a CUDA graph: write ``tokens`` / ``positions``, ``replay()``, which returns the
+    logits, or with ``greedy`` the next tokens.  With a paged cache a replay takes the pages it needs first; rows may be opened,
+    released and evicted between replays."""
 
-    def __init__(self, model: TensorParallelDecoder, batch: int) -> None:
-        self.model = model
+    def __init__(self, model: TensorParallelDecoder, batch: int, greedy: bool = False, rules: LogitRules | None = None) -> None:
+        self.model, self.batch = model, batch
         self.tokens = torch.zeros(batch, dtype=torch.int64, device=model.device)
         self.positions = torch.zeros(batch, dtype=torch.int32, device=model.device)
-        side = torch.cuda.Stream(device=model.device)
-        side.wait_stream(torch.cuda.current_stream(model.device))
-        with torch.cuda.stream(side):
-            for _ in range(2):  # warm up kernels, NCCL channels and the allocator before capturing
-                model.step(self.tokens, self.positions)
-            torch.cuda.synchronize(model.device)
-            self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph, stream=side):
-                self.logits = model.step(self.tokens, self.positions)
-        torch.cuda.current_stream(model.device).wait_stream(side)
+        with model.cache.idle() if model.cache is not None else nullcontext():
+            observed = None if rules is None else rules.lengths.clone()
+            side = torch.cuda.Stream(device=model.device)
+            side.wait_stream(torch.cuda.current_stream(model.device))
+            with torch.cuda.stream(side):
+                for _ in range(2):  # warm up kernels, NCCL channels and the allocator before capturing
+                    model.step(self.tokens, self.positions, greedy, rules)
+                torch.cuda.synchronize(model.device)
+                self.graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(self.graph, stream=side):
+                    self.logits = model.step(self.tokens, self.positions, greedy, rules)
+            torch.cuda.current_stream(model.device).wait_stream(side)
+            if rules is not None:
+                rules.lengths.copy_(observed)
         torch.cuda.synchronize(model.device)
 
     def replay(self) -> Tensor:
+        cache = self.model.cache
+        if cache is not None:
+            cache.prepare(self.batch)
         self.graph.replay()
+        if cache is not None:
+            cache.advance(self.batch)
         return self.logits
