@@ -167,6 +167,14 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
     return a.long_tokens ? __ldg(static_cast<const long long*>(a.tokens) + m * a.tokens_stride + i)
                          : __ldg(static_cast<const int*>(a.tokens) + m * a.tokens_stride + i);
   };
+  if (tracked) {
+    // the slice's logits come to L2 while the history is gathered
+    for (int block = threadIdx.x; block * kBlock < a.slice; block += kLogitThreads) {
+      const int from = max(place_of(block * kBlock), (shift + V - 1) / V * V), to = min(place_of(block * kBlock) + kBlock, end / V * V);
+      if (from < to)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row + from), "r"(uint32_t((to - from) * sizeof(T))) : "memory");
+    }
+  }
   for (int base = 0;; base += a.chunk) {
     const int last = min(base + a.chunk, a.slice);
     // the chunk's first logits, and their bits of the mask
