@@ -45,9 +45,9 @@ constexpr int kDeep = 2;                  // pieces of a thread under way
 constexpr int kSlots = 8192;              // of the hash table, at most; a power of two
 constexpr int kMost = 6144;               // tokens it takes, three quarters of its slots; more history than that goes by chunks of that many tokens
 constexpr int kRanks = 16;                // CTAs of a row, at most
-constexpr uint32_t kSeen = 0x80000000u;   // of a count: the token is in the prompt
-constexpr uint32_t kBiased = 0x40000000u; // of a count: the token has a bias
-constexpr uint32_t kCount = kBiased - 1;  // how often it was generated
+constexpr uint32_t kBiased = 0x80000000u; // of a count: the token has a bias
+constexpr uint32_t kSeen = 0x40000000u;   // of a count with kBiased: the token is in the history, as all without it are
+constexpr uint32_t kCount = kSeen - 1;  // how often it was generated
 constexpr uint32_t kNoPlace = 0xffffffffu;
 constexpr int64_t kNothing = -(int64_t(1) << 40);
 constexpr int kBiases = 512;              // entries of a chunk that are listed in shared memory
@@ -202,23 +202,14 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
       const uint32_t at = (block >> turn) * kBlock + uint32_t(place) % kBlock - uint32_t(base);
       return at < uint32_t(last - base) ? at : kNoPlace;
     };
-    // counts `add` for, or flags, the token at a place of the chunk
-    auto note = [&](uint32_t at, uint32_t add, uint32_t flag) {
+    // the table's slot of the token with a number, which it has from now on
+    auto slot_of = [&](uint32_t at) {
       uint32_t slot = (at + 1) * 2654435761u >> (__clz(a.slots) + 1);
-      for (;; slot = (slot + 1) & (a.slots - 1)) {
-        uint32_t key_there = *static_cast<volatile uint32_t*>(table_s + slot);
-        if (key_there == 0) {
-          key_there = atomicCAS(table_s + slot, 0u, at + 1);
-          if (key_there == 0) {
-            atomicOr(marked_s + at / 32, 1u << (at % 32));
-            break;
-          }
-        }
-        if (key_there == at + 1) break;
+      for (;;) {
+        const uint32_t there = atomicCAS(table_s + slot, 0u, at + 1);
+        if (there == 0 || there == at + 1) return slot;
+        slot = (slot + 1) & (a.slots - 1);
       }
-      if (flag) atomicOr(count_s + slot, flag);
-      else atomicAdd(count_s + slot, add);
-      return slot;
     };
     if (tracked) {
       for (int i = threadIdx.x * 4; i < 2 * a.slots + a.chunk / 32; i += kLogitThreads * 4) *reinterpret_cast<uint4*>(table_s + i) = make_uint4(0u, 0u, 0u, 0u);
@@ -226,17 +217,20 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
       __syncthreads();
       auto count = [&](int i, int64_t id) {
         const uint32_t at = number(id);
-        if (at != kNoPlace) note(at, 1u, i >= prompt ? 0u : kSeen);
+        if (at == kNoPlace) return;
+        atomicAdd(count_s + slot_of(at), i >= prompt ? 1u : 0u);
+        atomicOr(marked_s + at / 32, 1u << (at % 32));
       };
       int i = threadIdx.x;
       for (; i + 3 * kLogitThreads < length; i += 4 * kLogitThreads) {
         int64_t ids[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) ids[u] = history(i + u * kLogitThreads);
-#pragma unroll 1
-        for (int u = 0; u < 4; ++u) count(i + u * kLogitThreads, u == 0 ? ids[0] : u == 1 ? ids[1] : u == 2 ? ids[2] : ids[3]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) count(i + u * kLogitThreads, ids[u]);
       }
       for (; i < length; i += kLogitThreads) count(i, history(i));
+      __syncthreads();
     }
     // the biases of this chunk, in their order
     int biases = 0;
@@ -253,8 +247,19 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
         if (w < int(threadIdx.x >> 5)) slot += bias_count_s[w];
         biases += bias_count_s[w];
       }
+      // whether the history has the token: it is in the table before this group's entries come in, and if an entry of a group
+      // before brought it, that one's flag says so
+      bool seen = false;
       if (inside) {
-        const uint32_t there = note(at, 0u, kBiased);
+        uint32_t probe = (at + 1) * 2654435761u >> (__clz(a.slots) + 1);
+        while (table_s[probe] != 0 && table_s[probe] != at + 1) probe = (probe + 1) & (a.slots - 1);
+        seen = table_s[probe] != 0 && (count_s[probe] & (kBiased | kSeen)) != kBiased;
+      }
+      __syncthreads();
+      if (inside) {
+        const uint32_t there = slot_of(at);
+        atomicOr(count_s + there, seen ? kBiased | kSeen : kBiased);
+        atomicOr(marked_s + at / 32, 1u << (at % 32));
         if (slot < kBiases) {
           bias_slot_s[slot] = uint16_t(there);
           bias_at_s[slot] = int(at);
@@ -326,7 +331,7 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
         const int place = place_of(base + at);
         const int64_t id = token0 + place;
         float x = L::widen(row[place]);
-        if (count & (kSeen | kCount)) {
+        if ((count & (kBiased | kSeen)) != kBiased) {
           x = x > 0.f ? __fdiv_rn(x, repetition) : __fmul_rn(x, repetition);
           x = __fsub_rn(x, __fmul_rn(frequency, float(count & kCount)));
           if (count & kCount) x = __fsub_rn(x, presence);
