@@ -568,13 +568,21 @@ def tokens_of_keys(keys: Tensor) -> Tensor:
 # ---- operators over a paged cache, and on the logits ----
 
 _raw_stream = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream builds an object: 3 us of a call
-_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_current_device, _capturing = torch._C._cuda_getDevice, torch._C._cuda_isCurrentStreamCapturing
 
 
-@functools.lru_cache(maxsize=256)
-def _attention_workspace_bytes(index: int, *shape: int) -> int:
-    """Of the device that is current, ``index``."""
-    return _native.library().mkb_paged_attention_workspace_bytes(*shape)
+# What a call of these operators checks depends on the layouts of its tensors alone (shapes, strides, dtypes, devices) and on
+# plain numbers: calls whose layouts were checked before go straight to the C entry with the numbers made out then, which
+# checks pointers and alignment itself.  The checks took 5 of the 13 us of an attention call's host side.
+_Plan = tuple
+_plans: dict[tuple, _Plan] = {}
+
+
+def _planned(key: tuple, plan: _Plan) -> _Plan:
+    if len(_plans) >= 4096:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
 
 
 STATE_BYTES, STATES = 8192, 128     # of the attention over pages: zeroed words of one call at a time; states of a block
@@ -597,7 +605,7 @@ class _AttentionScratch:
         self.left = [self.blocks[-1].data_ptr() + i * STATE_BYTES for i in range(STATES)] + self.left
 
     def of(self, index: int, stream: int, need: int) -> tuple[int, Tensor]:
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing():
             workspace = torch.empty(need + STATE_BYTES, dtype=torch.uint8, device=index)
             if self.left:
                 return self.left.pop(), workspace
@@ -654,39 +662,60 @@ def paged_attention_decode(q: Tensor, lengths: Tensor, k_pages: Tensor, v_pages:
     (pools ``[pages, kv_heads, page, head_dim]``, page numbers ``tables`` int32 [rows, columns]) into ``out``.  An empty sequence
     and a row that is not in use (a negative length) give zeros.  ``weights`` (fp32 [pages, kv_heads, page]) adds up every
     slot's softmax weight over the query heads of its group."""
-    what, index = "paged_attention_decode", q.get_device()
-    if index < 0:
-        raise ValueError("mlkit_b200 kernels require CUDA tensors")
+    key = (q.shape, q.stride(), q.dtype, q.get_device(), lengths.shape, lengths.stride(), lengths.dtype, lengths.get_device(),
+           k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape, v_pages.stride(), v_pages.dtype,
+           v_pages.get_device(), tables.shape, tables.stride(), tables.dtype, tables.get_device(), out.shape, out.stride(), out.dtype,
+           out.get_device(), scale, None if weights is None else
+           (weights.shape, weights.stride(), weights.dtype, weights.get_device()))
+    index, function, need, numbers = _plans.get(key) or _planned(key, _plan_attention(q, lengths, k_pages, v_pages, tables, out,
+                                                                                     scale, weights))
     if _current_device() != index:
         with torch.cuda.device(index):
             return paged_attention_decode(q, lengths, k_pages, v_pages, tables, out, scale=scale, weights=weights)
-    dtype = q.dtype
+    stream = _raw_stream(index)
+    state, workspace = _scratch(index, stream, need)
+    status = function(q.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), out.data_ptr(),
+                      None if weights is None else weights.data_ptr(), *numbers, state, workspace.data_ptr(), need, stream)
+    if status:
+        _native.check(status, "paged_attention_decode")
+
+
+def _plan_attention(q: Tensor, lengths: Tensor, k_pages: Tensor, v_pages: Tensor, tables: Tensor, out: Tensor, scale: float | None,
+                    weights: Tensor | None) -> _Plan:
+    what, index, dtype = "paged_attention_decode", q.get_device(), q.dtype
+    if index < 0:
+        raise ValueError("mlkit_b200 kernels require CUDA tensors")
     if q.dim() != 3 or k_pages.dtype is not dtype:
         raise ValueError(f"{what}: queries are [rows, q_heads, head_dim] in the dtype of the pages")
     rows, q_heads, head_dim = q.shape
     row, head, step = q.stride()
     _check_pages(what, index, k_pages, v_pages, weights, tables)
-    pages, kv_heads, page, width = k_pages.shape
-    if step != 1 or width != head_dim:
-        raise ValueError(f"{what}: queries have contiguous heads of {width}")
+    if step != 1 or k_pages.shape[3] != head_dim:
+        raise ValueError(f"{what}: queries have contiguous heads of {k_pages.shape[3]}")
+    _check_out(what, index, out, dtype, rows, q_heads, head_dim, tables)
+    _check_rows(what, index, rows, lengths)
+    return _attention_plan(index, "mkb_paged_attention_decode", q_heads, k_pages, tables, (row, head), (), scale, weights)
+
+
+def _check_out(what: str, index: int, out: Tensor, dtype: torch.dtype, rows: int, q_heads: int, head_dim: int, tables: Tensor) -> None:
     if (out.dtype is not dtype or out.numel() != rows * q_heads * head_dim or not out.is_contiguous() or out.get_device() != index
             or out.dim() < 2 or out.shape[0] != rows):
         raise ValueError(f"{what}: the output is a contiguous [rows, q_heads, head_dim] in the dtype and on the device of the queries")
-    _check_rows(what, index, rows, lengths)
-    columns = tables.shape[1]
     if tables.shape[0] != rows:
         raise ValueError(f"{what}: a row of tables for each row of queries")
-    need = _attention_workspace_bytes(index, rows, q_heads, kv_heads, head_dim, page, columns, weights is not None)
-    stream = _raw_stream(index)
-    state, workspace = _scratch(index, stream, need)
-    by_page, by_head, by_slot, _ = k_pages.stride()
-    status = _native.library().mkb_paged_attention_decode(
-        q.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), out.data_ptr(),
-        None if weights is None else weights.data_ptr(), rows, q_heads, kv_heads, head_dim, page, columns, pages, by_page, by_head,
-        by_slot, tables.stride(0), row, head, head_dim ** -0.5 if scale is None else scale, _tag(dtype, "cache"),
-        state, workspace.data_ptr(), need, stream)
-    if status:
-        _native.check(status, what)
+
+
+def _attention_plan(index: int, entry: str, q_heads: int, k_pages: Tensor, tables: Tensor, q_strides: tuple[int, ...],
+                    theta: tuple[float, ...], scale: float | None, weights: Tensor | None) -> _Plan:
+    """``(device, C entry, bytes of workspace, the entry's numbers)``."""
+    pages, kv_heads, page, head_dim = k_pages.shape
+    rows, columns = tables.shape
+    library = _native.library()
+    with torch.cuda.device(index):
+        need = library.mkb_paged_attention_workspace_bytes(rows, q_heads, kv_heads, head_dim, page, columns, weights is not None)
+    return (index, getattr(library, entry), need,
+            (rows, q_heads, kv_heads, head_dim, page, columns, pages, *k_pages.stride()[:3], tables.stride(0), *q_strides, *theta,
+             head_dim ** -0.5 if scale is None else scale, _tag(k_pages.dtype, "cache")))
 
 
 def paged_rope_attention_decode(qkv: Tensor, positions: Tensor, lengths: Tensor, k_pages: Tensor, v_pages: Tensor, tables: Tensor,
@@ -696,41 +725,46 @@ def paged_rope_attention_decode(qkv: Tensor, positions: Tensor, lengths: Tensor,
     stored with its value in slot ``lengths`` of the sequence, and the rotated queries attend to slots ``0..lengths``.  ``qkv`` is
     left unrotated, ``lengths`` as they are; a row with a negative length is not in use (zeros, nothing stored).  Positions
     and lengths differ where slots were evicted.  ``weights`` as in ``paged_attention_decode``; a new slot begins at zero."""
-    what, index = "paged_rope_attention_decode", qkv.get_device()
-    if index < 0:
-        raise ValueError("mlkit_b200 kernels require CUDA tensors")
+    key = (qkv.shape, qkv.stride(), qkv.dtype, qkv.get_device(), positions.shape, positions.stride(), positions.dtype,
+           positions.get_device(), lengths.shape, lengths.stride(), lengths.dtype, lengths.get_device(), k_pages.shape,
+           k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape, v_pages.stride(), v_pages.dtype,
+           v_pages.get_device(), tables.shape, tables.stride(), tables.dtype, tables.get_device(), out.shape, out.stride(), out.dtype,
+           out.get_device(), q_heads, kv_heads, head_dim, theta, scale, None if weights is None else
+           (weights.shape, weights.stride(), weights.dtype, weights.get_device()))
+    index, function, need, numbers = _plans.get(key) or _planned(
+        key, _plan_rope_attention(qkv, positions, lengths, k_pages, v_pages, tables, out, q_heads, kv_heads, head_dim, theta, scale,
+                                  weights))
     if _current_device() != index:
         with torch.cuda.device(index):
             return paged_rope_attention_decode(qkv, positions, lengths, k_pages, v_pages, tables, out, q_heads=q_heads,
                                                kv_heads=kv_heads, head_dim=head_dim, theta=theta, scale=scale, weights=weights)
-    dtype = qkv.dtype
+    stream = _raw_stream(index)
+    state, workspace = _scratch(index, stream, need)
+    status = function(qkv.data_ptr(), positions.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                      tables.data_ptr(), out.data_ptr(), None if weights is None else weights.data_ptr(), *numbers, state,
+                      workspace.data_ptr(), need, stream)
+    if status:
+        _native.check(status, "paged_rope_attention_decode")
+
+
+def _plan_rope_attention(qkv: Tensor, positions: Tensor, lengths: Tensor, k_pages: Tensor, v_pages: Tensor, tables: Tensor,
+                         out: Tensor, q_heads: int, kv_heads: int, head_dim: int, theta: float, scale: float | None,
+                         weights: Tensor | None) -> _Plan:
+    what, index, dtype = "paged_rope_attention_decode", qkv.get_device(), qkv.dtype
+    if index < 0:
+        raise ValueError("mlkit_b200 kernels require CUDA tensors")
     if qkv.dim() != 2 or k_pages.dtype is not dtype:
         raise ValueError(f"{what}: q | k | v is [rows, (q_heads + 2 * kv_heads) * head_dim] in the dtype of the pages")
     rows, width = qkv.shape
     row, step = qkv.stride()
     _check_pages(what, index, k_pages, v_pages, weights, tables)
-    pages, heads, page, depth = k_pages.shape
+    _, heads, _, depth = k_pages.shape
     if step != 1 or heads != kv_heads or depth != head_dim or width != (q_heads + 2 * kv_heads) * head_dim:
         raise ValueError(f"{what}: rows of {width} values and pages of {heads} heads of {depth} are not {q_heads} query and "
                          f"{kv_heads} key-value heads of {head_dim}")
-    if (out.dtype is not dtype or out.numel() != rows * q_heads * head_dim or not out.is_contiguous() or out.get_device() != index
-            or out.dim() < 2 or out.shape[0] != rows):
-        raise ValueError(f"{what}: the output is a contiguous [rows, q_heads, head_dim] in the dtype and on the device of the queries")
+    _check_out(what, index, out, dtype, rows, q_heads, head_dim, tables)
     _check_rows(what, index, rows, positions, lengths)
-    columns = tables.shape[1]
-    if tables.shape[0] != rows:
-        raise ValueError(f"{what}: a row of tables for each row of queries")
-    need = _attention_workspace_bytes(index, rows, q_heads, kv_heads, head_dim, page, columns, weights is not None)
-    stream = _raw_stream(index)
-    state, workspace = _scratch(index, stream, need)
-    by_page, by_head, by_slot, _ = k_pages.stride()
-    status = _native.library().mkb_paged_rope_attention_decode(
-        qkv.data_ptr(), positions.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(),
-        out.data_ptr(), None if weights is None else weights.data_ptr(), rows, q_heads, kv_heads, head_dim, page, columns, pages,
-        by_page, by_head, by_slot, tables.stride(0), row, theta, head_dim ** -0.5 if scale is None else scale, _tag(dtype, "cache"),
-        state, workspace.data_ptr(), need, stream)
-    if status:
-        _native.check(status, what)
+    return _attention_plan(index, "mkb_paged_rope_attention_decode", q_heads, k_pages, tables, (row,), (theta,), scale, weights)
 
 
 def evict_pages(k_pages: Tensor, v_pages: Tensor, weights: Tensor, tables: Tensor, lengths: Tensor, new_tables: Tensor, *,
@@ -739,30 +773,39 @@ def evict_pages(k_pages: Tensor, v_pages: Tensor, weights: Tensor, tables: Tenso
     heaviest of the others by ``weights`` (a tie to the lower slot).  They are copied, in slot order, to the pages that
     ``new_tables`` names; these must be named once and be none of ``tables``.  Returns the kept slots, int32 [rows, kv_heads,
     budget], -1 behind the last.  The caller swaps the tables, sets the lengths and frees the old pages."""
-    what, index = "evict_pages", k_pages.get_device()
-    if index < 0:
-        raise ValueError("mlkit_b200 kernels require CUDA tensors")
+    key = (k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape, v_pages.stride(), v_pages.dtype,
+           v_pages.get_device(), weights.shape, weights.stride(), weights.dtype, weights.get_device(), tables.shape, tables.stride(),
+           tables.dtype, tables.get_device(), lengths.shape, lengths.stride(), lengths.dtype, lengths.get_device(), new_tables.shape,
+           new_tables.stride(), new_tables.dtype, new_tables.get_device(), budget, sinks, recent)
+    index, function, shape, numbers = _plans.get(key) or _planned(key, _plan_evict(k_pages, v_pages, weights, tables, lengths,
+                                                                                  new_tables, budget, sinks, recent))
     if _current_device() != index:
         with torch.cuda.device(index):
             return evict_pages(k_pages, v_pages, weights, tables, lengths, new_tables, budget=budget, sinks=sinks, recent=recent)
+    kept = tables.new_empty(shape)
+    status = function(k_pages.data_ptr(), v_pages.data_ptr(), weights.data_ptr(), tables.data_ptr(), lengths.data_ptr(),
+                      new_tables.data_ptr(), kept.data_ptr(), *numbers, _raw_stream(index))
+    if status:
+        _native.check(status, "evict_pages")
+    return kept
+
+
+def _plan_evict(k_pages: Tensor, v_pages: Tensor, weights: Tensor, tables: Tensor, lengths: Tensor, new_tables: Tensor, budget: int,
+                sinks: int, recent: int) -> _Plan:
+    what, index = "evict_pages", k_pages.get_device()
+    if index < 0:
+        raise ValueError("mlkit_b200 kernels require CUDA tensors")
     _check_pages(what, index, k_pages, v_pages, weights, tables, new_tables)
-    pages, kv_heads, page, head_dim = k_pages.shape
-    _tag(k_pages.dtype, "cache")
-    if k_pages.dtype is torch.float32:
+    if k_pages.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"{what}: pages are fp16 or bf16")
+    pages, kv_heads, page, head_dim = k_pages.shape
     rows, columns = tables.shape
     if new_tables.shape[0] != rows:
         raise ValueError(f"{what}: a row of new tables for each row of tables")
     _check_rows(what, index, rows, lengths)
-    kept = torch.empty((rows, kv_heads, max(budget, 0)), dtype=torch.int32, device=index)
-    by_page, by_head, by_slot, _ = k_pages.stride()
-    status = _native.library().mkb_paged_evict(
-        k_pages.data_ptr(), v_pages.data_ptr(), weights.data_ptr(), tables.data_ptr(), lengths.data_ptr(), new_tables.data_ptr(),
-        kept.data_ptr(), rows, kv_heads, head_dim, page, columns, new_tables.shape[1], pages, by_page, by_head, by_slot,
-        tables.stride(0), new_tables.stride(0), budget, sinks, recent, _raw_stream(index))
-    if status:
-        _native.check(status, what)
-    return kept
+    return (index, _native.library().mkb_paged_evict, (rows, kv_heads, max(budget, 0)),
+            (rows, kv_heads, head_dim, page, columns, new_tables.shape[1], pages, *k_pages.stride()[:3], tables.stride(0),
+             new_tables.stride(0), budget, sinks, recent))
 
 
 def adjust_logits(logits: Tensor, *, tokens: Tensor | None = None, lengths: Tensor | None = None, prompts: Tensor | None = None,
@@ -779,59 +822,64 @@ def adjust_logits(logits: Tensor, *, tokens: Tensor | None = None, lengths: Tens
 
     Ids outside ``offset..offset + width`` (-1 fills a row up) have no effect.  ``best`` (int64 [rows]) receives the words of
     ``argmax_keys`` for the result, ``picked`` (int64 [rows]) its greedy tokens."""
-    what, index = "adjust_logits", logits.get_device()
-    if index < 0:
-        raise ValueError("mlkit_b200 kernels require CUDA tensors")
+    if out is None:
+        out = logits
+    given = (logits, out, tokens, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, mask, best, picked)
+    key = (offset, *[None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in given])
+    index, function, numbers = _plans.get(key) or _planned(key, _plan_logits(*given, offset))
     if _current_device() != index:
         with torch.cuda.device(index):
             return adjust_logits(logits, tokens=tokens, lengths=lengths, prompts=prompts, repetition=repetition, frequency=frequency,
                                  presence=presence, bias_tokens=bias_tokens, bias=bias, mask=mask, offset=offset, best=best,
                                  picked=picked, out=out)
+    status = function(*[None if t is None else t.data_ptr() for t in given], *numbers, _raw_stream(index))
+    if status:
+        _native.check(status, "adjust_logits")
+    return out
+
+
+def _plan_logits(logits: Tensor, out: Tensor, tokens: Tensor | None, lengths: Tensor | None, prompts: Tensor | None,
+                 repetition: Tensor | None, frequency: Tensor | None, presence: Tensor | None, bias_tokens: Tensor | None,
+                 bias: Tensor | None, mask: Tensor | None, best: Tensor | None, picked: Tensor | None, offset: int) -> _Plan:
+    what, index = "adjust_logits", logits.get_device()
+    if index < 0:
+        raise ValueError("mlkit_b200 kernels require CUDA tensors")
     if logits.dim() != 2 or logits.stride(1) != 1:
         raise ValueError(f"{what}: logits are [rows, width] with contiguous rows")
     rows, width = logits.shape
-    dtype, row = logits.dtype, logits.stride(0)
-    if out is None:
-        out = logits
-    elif out.shape != logits.shape or out.dtype is not dtype or out.stride(1) != 1 or out.get_device() != index:
+    if out.shape != logits.shape or out.dtype is not logits.dtype or out.stride(1) != 1 or out.get_device() != index:
         raise ValueError(f"{what}: the output matches the logits in shape, dtype and device, with contiguous rows")
 
-    def vector(name: str, given: Tensor | None, kind: torch.dtype) -> int | None:
-        if given is None:
-            return None
-        if given.dtype is not kind or given.dim() != 1 or given.shape[0] != rows or not given.is_contiguous() or given.get_device() != index:
+    def vector(name: str, given: Tensor | None, kind: torch.dtype) -> None:
+        if given is not None and (given.dtype is not kind or given.dim() != 1 or given.shape[0] != rows or not given.is_contiguous()
+                                  or given.get_device() != index):
             raise ValueError(f"{what}: {name} must be a contiguous {kind} vector of {rows} rows on the device of the logits")
-        return given.data_ptr()
 
-    def table(name: str, given: Tensor | None, *kinds: torch.dtype) -> tuple[int | None, int, int]:
+    def table(name: str, given: Tensor | None, *kinds: torch.dtype) -> tuple[int, int]:
         if given is None:
-            return None, 0, 0
+            return 0, 0
         if given.dim() != 2 or given.shape[0] != rows or given.dtype not in kinds or given.get_device() != index:
             raise ValueError(f"{what}: {name} must be {kinds[0]} [rows, entries] on the device of the logits")
         stride, step = given.stride()
         if step != 1 and given.shape[1] > 1:
             raise ValueError(f"{what}: {name} must have contiguous rows")
-        return given.data_ptr(), given.shape[1], stride
+        return given.shape[1], stride
 
-    history, held, history_stride = table("tokens", tokens, torch.int64, torch.int32)
+    for name, given, kind in (("lengths", lengths, torch.int32), ("prompts", prompts, torch.int32),
+                              ("repetition", repetition, torch.float32), ("frequency", frequency, torch.float32),
+                              ("presence", presence, torch.float32), ("best", best, torch.int64), ("picked", picked, torch.int64)):
+        vector(name, given, kind)
+    history = table("tokens", tokens, torch.int64, torch.int32)
     if (tokens is None) != (lengths is None):
         raise ValueError(f"{what}: a history needs its lengths")
     if tokens is None and not (prompts is None and repetition is None and frequency is None and presence is None):
         raise ValueError(f"{what}: penalties need a history of tokens")
-    entries, biases, bias_stride = table("bias_tokens", bias_tokens, torch.int32)
-    values, count, stride = table("bias", bias, torch.float32)
-    if (bias is None) != (bias_tokens is None) or count != biases or stride != bias_stride:
+    biases = table("bias_tokens", bias_tokens, torch.int32)
+    if (bias is None) != (bias_tokens is None) or table("bias", bias, torch.float32) != biases:
         raise ValueError(f"{what}: biases need a token for every value, in the same layout")
-    bits, words, mask_stride = table("mask", mask, torch.int32)
-    status = _native.library().mkb_adjust_logits(
-        logits.data_ptr(), out.data_ptr(), history, vector("lengths", lengths, torch.int32), vector("prompts", prompts, torch.int32),
-        vector("repetition", repetition, torch.float32), vector("frequency", frequency, torch.float32),
-        vector("presence", presence, torch.float32), entries, values, bits, vector("best", best, torch.int64),
-        vector("picked", picked, torch.int64), rows, width, row, out.stride(0), held, history_stride, biases, bias_stride, words,
-        mask_stride, offset, tokens is not None and tokens.dtype is torch.int64, _tag(dtype, "logit"), _raw_stream(index))
-    if status:
-        _native.check(status, what)
-    return out
+    return (index, _native.library().mkb_adjust_logits,
+            (rows, width, logits.stride(0), out.stride(0), *history, *biases, *table("mask", mask, torch.int32), offset,
+             tokens is not None and tokens.dtype is torch.int64, _tag(logits.dtype, "logit")))
 
 
 def decode_status() -> int:
