@@ -346,12 +346,14 @@ int mkb_argmax(const void* logits, void* best, int M, int64_t width, int64_t row
  *     is empty.  q is [M, q_heads, head_dim] with strides of whole 16-byte vectors; out is contiguous.
  * mkb_paged_rope_attention_decode: qkv[m] = [q_heads | kv_heads | kv_heads] x head_dim; the new key is rotated by
  *     positions[m] (rotate-half pairing, angle position * theta^(-2i/head_dim)) and stored with the value at slot lengths[m];
- *     the rotated queries (not rounded) attend to slots 0..lengths[m].  The caller advances lengths.  A slot that the
- *     call writes belongs to one sequence only.
+ *     the rotated queries (not rounded) attend to slots 0..lengths[m].  The caller advances lengths.  The page of a new
+ *     token belongs to one sequence only; pages that are only read may be in several tables.
  * weights (fp32 [pages, kv_heads, page], contiguous, may be null): every slot's softmax weight, summed over the query heads
- *     that share its key-value head, is added; the slot of a new token begins at zero.
- * head_dim 64, 128, 192 or 256; any number of query heads per key-value head.  What lies in slots behind a sequence's
- * length is never used.  A length beyond the table, and an entry that is no page of the pool, never become an address:
+ *     that share its key-value head, is added; the slot of a new token begins at zero.  With weights no page is in two
+ *     sequences' tables, nor twice in one: their additions would meet.
+ * head_dim 64, 128, 192 or 256; any number of query heads per key-value head.  out may be q itself, and overlaps it in no
+ * other way.  What lies in slots behind a sequence's length is never used; queries, keys and values in use are finite (an
+ * infinity may give NaN where it need not: weights and rotated queries are held as two 16-bit parts).  A length beyond the table, and an entry that is no page of the pool, never become an address:
  * such slots are left out and mkb_decode_status is raised.
  * state: MKB_PAGED_STATE_BYTES bytes that are zero before the first call that uses them; every call leaves them zero.
  * workspace: mkb_paged_attention_workspace_bytes bytes (16-byte aligned), of no meaning before and after the call.
@@ -384,15 +386,15 @@ int mkb_paged_evict(void* k_pages, void* v_pages, float* weights, const int* tab
                     int64_t new_table_stride, int budget, int sinks, int recent, void* stream);
 /*
  * Penalties, biases and a mask on logits [M, width] (dtype MKB_F16/BF16/F32, rows logits_stride apart) of the tokens
- * offset .. offset + width, into out (may be logits itself).  For token v of row m, in fp32 in this order, rounded once:
+ * offset .. offset + width, into out (may be logits itself, and overlaps them in no other way).  For token v of row m, in fp32 in this order, rounded once:
  *   v in tokens[m, 0..lengths[m]):                        x = x > 0 ? x / repetition[m] : x * repetition[m]
  *   c times in tokens[m, prompts[m]..lengths[m]):         x -= frequency[m] * c;  x -= presence[m] when c > 0
  *   entries e with bias_tokens[m, e] == v:                x += the sum of bias[m, e]
  *   bit v % 32 of mask[m, v / 32] is 0:                   x = -infinity
  * Each part is left out when its pointer is null (prompts: nothing is prompt; repetition: 1; frequency, presence: 0).
  * tokens are int32, or int64 with long_tokens; ids outside this width (a negative one fills a row up) have no effect;
- * lengths beyond `history` count as `history`.  best[m] (uint64, may be null): the word mkb_argmax gives for the result, with a
- * 32-bit key for fp32; picked[m] (int64, may be null): the token of the largest result, the smallest on a tie.
+ * lengths beyond `history` count as `history`.  best[m] (uint64, may be null): the word mkb_argmax gives for the result (a
+ * negative zero counting as zero), with a 32-bit key for fp32; picked[m] (int64, may be null): the token of the largest result, the smallest on a tie.
  */
 int mkb_adjust_logits(const void* logits, void* out, const void* tokens, const int* lengths, const int* prompts,
                       const float* repetition, const float* frequency, const float* presence, const int* bias_tokens,

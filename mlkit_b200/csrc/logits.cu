@@ -458,6 +458,10 @@ extern "C" int mkb_adjust_logits(const void* logits, void* out, const void* toke
   if (M == 0) return MKB_OK;
   MKB_REQUIRE(logits && out, MKB_E_ARGUMENT, "adjust_logits: null pointer");
   MKB_REQUIRE(M == 1 || out_stride >= width, MKB_E_ARGUMENT, "adjust_logits: rows of the output overlap");
+  const int64_t size = dtype_bytes(dtype);
+  MKB_REQUIRE((logits == out && (M == 1 || logits_stride == out_stride)) ||
+                  !overlap(logits, ((M - 1) * logits_stride + width) * size, out, ((M - 1) * out_stride + width) * size),
+              MKB_E_ARGUMENT, "adjust_logits: the output overlaps the logits");
   MKB_REQUIRE(!tokens || history == 0 || lengths, MKB_E_ARGUMENT, "adjust_logits: a history needs its lengths");
   MKB_REQUIRE((bias_tokens != nullptr) == (bias != nullptr), MKB_E_ARGUMENT, "adjust_logits: biases need tokens and values");
   MKB_REQUIRE(!mask || (mask_words << 5) >= offset + width, MKB_E_ARGUMENT, "adjust_logits: a mask of %lld words ends before token %lld",

@@ -28,6 +28,12 @@ int cuda_fail(cudaError_t status, const char* what);
     if (status_ != cudaSuccess) return ::mkb::cuda_fail(status_, what); \
   } while (0)
 
+// Whether [a, a + a_bytes) and [b, b + b_bytes) share a byte.
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + uintptr_t(b_bytes) && y < x + uintptr_t(a_bytes);
+}
+
 // ---- device properties, cached per device ---------------------------------------------------
 struct DeviceInfo {
   int sm_count;

@@ -789,6 +789,11 @@ int attend(const char* what, AttentionArguments& a, bool rope, void* out, float*
               MKB_E_ALIGNMENT, "%s: queries and outputs lie on 16-byte vectors", what);
   MKB_REQUIRE(int64_t(M) * kv_heads * ((q_heads / kv_heads + kHeads - 1) / kHeads) * ((int64_t(columns) * page + kTile - 1) / kTile) < (int64_t(1) << 31),
               MKB_E_UNSUPPORTED, "%s: %d sequences of %d pages of %d slots", what, M, columns, page);
+  const int64_t out_row = int64_t(q_heads) * head_dim, q_width = rope ? (int64_t(q_heads) + 2 * kv_heads) * head_dim : (q_heads - 1) * a.q_head + head_dim;
+  const bool in_place = !rope && out == a.q && a.q_head == head_dim && (M == 1 || a.q_row == out_row);
+  MKB_REQUIRE(a.q_row >= 0 && a.q_head >= 0, MKB_E_ARGUMENT, "%s: negative stride", what);
+  MKB_REQUIRE(in_place || !overlap(a.q, ((M - 1) * a.q_row + q_width) * 2, out, M * out_row * 2), MKB_E_ARGUMENT,
+              "%s: the output overlaps the queries", what);
   const Workspace parts(M, q_heads, kv_heads, head_dim, page, columns, weights != nullptr);
   MKB_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= parts.bytes, MKB_E_ARGUMENT,
               "%s: workspace of %lld bytes, %lld needed", what, (long long)workspace_bytes, (long long)parts.bytes);

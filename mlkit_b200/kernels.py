@@ -661,7 +661,7 @@ def paged_attention_decode(q: Tensor, lengths: Tensor, k_pages: Tensor, v_pages:
     """Attention of one query token per sequence (``q`` [rows, q_heads, head_dim]) to the ``lengths`` slots of its paged cache
     (pools ``[pages, kv_heads, page, head_dim]``, page numbers ``tables`` int32 [rows, columns]) into ``out``.  An empty sequence
     and a row that is not in use (a negative length) give zeros.  ``weights`` (fp32 [pages, kv_heads, page]) adds up every
-    slot's softmax weight over the query heads of its group."""
+    slot's softmax weight over the query heads of its group; no page is then in the tables twice, as it may be without."""
     key = (q.shape, q.stride(), q.dtype, q.get_device(), lengths.shape, lengths.stride(), lengths.dtype, lengths.get_device(),
            k_pages.shape, k_pages.stride(), k_pages.dtype, k_pages.get_device(), v_pages.shape, v_pages.stride(), v_pages.dtype,
            v_pages.get_device(), tables.shape, tables.stride(), tables.dtype, tables.get_device(), out.shape, out.stride(), out.dtype,

@@ -320,6 +320,79 @@ def test_streams_and_graphs_that_overlap():
             c["held"].sub_(7)
 
 
+def test_captured_calls_when_no_cleared_state_is_left(monkeypatch):
+    """Their graphs clear one of their own; and a captured call never shares one with another."""
+    lengths = [3000, 40]
+    keys, values, tables, weights = make_cache(lengths, kv_heads=1, head_dim=64, page=16, dtype=HALF)
+    q, held = torch.randn(2, 8, 64).half().cuda(), torch.tensor(lengths, dtype=torch.int32).cuda()
+    pool = (held, keys.cuda(), values.cuda(), tables.cuda())
+    expected = torch.empty_like(q)
+    kernels.paged_attention_decode(q, *pool, expected)
+    scratch = kernels._attention_scratch[q.device.index]
+    outs, graphs, side, left = [], [], torch.cuda.Stream(), len(scratch.left)
+    for attempt in range(4):
+        if attempt == 2:
+            monkeypatch.setattr(scratch, "left", [])
+        outs.append(torch.empty_like(q))
+        graphs.append(torch.cuda.CUDAGraph())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graphs[-1], stream=side):
+            kernels.paged_attention_decode(q, *pool, outs[-1])
+        if attempt < 2:
+            assert len(scratch.left) == left - attempt - 1
+    for _ in range(20):
+        for graph, stream in zip(graphs, [torch.cuda.Stream() for _ in graphs]):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, expected) for out in outs)
+
+
+def test_attention_in_place():
+    lengths = [2500, 3, 0, 90]
+    keys, values, tables, _ = make_cache(lengths, kv_heads=2, head_dim=128, page=16, dtype=HALF)
+    q = torch.randn(4, 8, 128).half().cuda()
+    pool = (torch.tensor(lengths, dtype=torch.int32).cuda(), keys.cuda(), values.cuda(), tables.cuda())
+    out = torch.empty_like(q)
+    kernels.paged_attention_decode(q, *pool, out)
+    kernels.paged_attention_decode(q, *pool, q)
+    assert torch.equal(q, out)
+
+
+def test_sequences_that_share_pages():
+    """A common prefix is in two tables: read by both, written by neither."""
+    keys, values, tables, _ = make_cache([40, 40], kv_heads=1, head_dim=64, page=16, dtype=HALF)
+    tables[1, :2] = tables[0, :2]
+    q = torch.randn(2, 4, 64).half()
+    out = torch.empty(2, 4, 64, dtype=HALF, device="cuda")
+    kernels.paged_attention_decode(q.cuda(), torch.tensor([40, 40], dtype=torch.int32).cuda(), keys.cuda(), values.cuda(), tables.cuda(), out)
+    for row in (0, 1):
+        expected, bound, _, _ = attend(q[row].double(), slots_of(keys, tables[row], 40), slots_of(values, tables[row], 40), 0.125, HALF, False)
+        assert ((out.cpu().double()[row] - expected).abs() <= bound).all()
+
+
+def test_layouts_are_told_apart():
+    """Calls of one shape and other strides, types or tables, in turn: none takes another's checked layout."""
+    lengths = [33, 70]
+    for attempt in range(2):
+        for dtype, slots_first, columns in ((HALF, False, None), (BRAIN, False, None), (HALF, True, None), (HALF, False, 9), (HALF, False, None)):
+            check_read(lengths, 4, 2, 64, 16, dtype, slots_first=slots_first, columns=columns, weigh=attempt == 1)
+    q, pages = torch.zeros(2, 4, 64, dtype=HALF, device="cuda"), torch.zeros(9, 2, 16, 64, dtype=HALF, device="cuda")
+    tables, held = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    good = dict(q=q, lengths=held, k_pages=pages, v_pages=pages.clone(), tables=tables, out=torch.empty_like(q))
+    kernels.paged_attention_decode(**good)
+    for name, bad in (("q", q.to(BRAIN)), ("q", q[:, :, ::2]), ("lengths", held.long()), ("lengths", held[:1]), ("k_pages", pages.to(BRAIN)),
+                      ("v_pages", pages[:8]), ("v_pages", pages.permute(0, 1, 3, 2)), ("tables", tables.long()), ("tables", tables[:1]),
+                      ("tables", tables.t().contiguous().t()), ("out", q[:1]), ("out", q.float()), ("out", q.cpu()), ("lengths", held.cpu()),
+                      ("tables", tables.cpu()), ("k_pages", pages.cpu())):
+        for _ in range(2):
+            with pytest.raises(ValueError):
+                kernels.paged_attention_decode(**(good | {name: bad}))
+    for weights in (torch.zeros(9, 2, 16, dtype=HALF, device="cuda"), torch.zeros(9, 2, 15, device="cuda"), torch.zeros(9, 2, 16)):
+        with pytest.raises(ValueError):
+            kernels.paged_attention_decode(**good, weights=weights)
+
+
 def test_pools_whose_offsets_pass_32_bits():
     """Elements beyond 2^32 bytes and 2^31 elements: the last pages of a pool of 2^32 + bytes."""
     page, heads, width = 256, 8, 128

@@ -10,7 +10,7 @@ POINTER = 1 << 20
 ARGUMENT, UNSUPPORTED, ALIGNMENT, CUDA = -1, -2, -3, -4
 needs_no_device = pytest.mark.skipif(torch.cuda.is_available(), reason="an accepted call would launch on made-up addresses")
 
-READ = dict(q=POINTER, lengths=POINTER, k=POINTER, v=POINTER, tables=POINTER, out=POINTER, weights=None, rows=2, q_heads=8, kv_heads=2,
+READ = dict(q=POINTER, lengths=POINTER, k=POINTER, v=POINTER, tables=POINTER, out=2 * POINTER, weights=None, rows=2, q_heads=8, kv_heads=2,
             head_dim=128, page=16, columns=4, pages=10, page_stride=2 * 16 * 128, head_stride=16 * 128, slot_stride=128,
             table_stride=4, q_row=8 * 128, q_head=128, scale=0.1, dtype=F16, state=POINTER, workspace=POINTER, size=1 << 40, stream=None)
 EVICT = dict(k=POINTER, v=POINTER, weights=POINTER, tables=POINTER, lengths=POINTER, new=POINTER, kept=POINTER, rows=2, kv_heads=2,
@@ -62,10 +62,22 @@ def test_attention_refuses(call):
             (UNSUPPORTED, [{"dtype": F32}, {"dtype": 9}, {"head_dim": 32}, {"head_dim": 96}, {"head_dim": 320}, {"rows": 70000},
                            {"columns": 1 << 20, "page": 1 << 10}, {"pages": 1 << 30, "page_stride": 1 << 20}]),
             (ARGUMENT, [{"workspace": POINTER + 8}]),
-            (ALIGNMENT, [{"q": POINTER + 2}, {"k": POINTER + 8}, {"v": POINTER + 8}, {"out": POINTER + 8}, {"slot_stride": 132},
+            (ALIGNMENT, [{"q": POINTER + 2}, {"k": POINTER + 8}, {"v": POINTER + 8}, {"out": 2 * POINTER + 8}, {"slot_stride": 132},
                          {"page_stride": 4100}, {"head_stride": 2052}, {"q_row": 1028}])):
         for changed in changes:
             assert call(**changed) == code, (changed, _native.library().mkb_last_error())
+
+
+@needs_no_device
+def test_outputs_that_overlap():
+    row = 8 * 128 * 2
+    assert read(out=POINTER) == CUDA                                        # in place
+    assert read(out=POINTER, q_row=8 * 128 + 64) == ARGUMENT and read(out=POINTER, q_head=256, q_row=2048) == ARGUMENT
+    assert read(out=POINTER + row) == ARGUMENT and read(out=POINTER - row) == ARGUMENT
+    assert read(out=POINTER + 2 * row) == CUDA and read(out=POINTER - 2 * row) == CUDA
+    qkv = 12 * 128 * 2
+    assert rope(out=POINTER, q_row=qkv // 2) == ARGUMENT and rope(out=POINTER + 2 * qkv, q_row=qkv // 2) == CUDA
+    assert adjust(out=POINTER + 2000) == ARGUMENT and adjust(out=POINTER + 4000) == CUDA and adjust(out=POINTER, out_stride=1001) == ARGUMENT
 
 
 @needs_no_device
@@ -87,7 +99,7 @@ def test_eviction_takes_and_refuses():
 
 @needs_no_device
 def test_logits_taken_and_refused():
-    for changed in ({}, {"dtype": F32}, {"tokens": None, "lengths": None}, {"mask": POINTER, "words": 32}, {"stride": 0},
+    for changed in ({}, {"dtype": F32}, {"tokens": None, "lengths": None}, {"mask": POINTER, "words": 32}, {"stride": 0, "out": 2 * POINTER},
                     {"bias": POINTER, "bias_tokens": POINTER, "biases": 3}, {"history": 0, "lengths": None}):
         assert adjust(**changed) == CUDA, changed
     assert adjust(rows=0) == 0
