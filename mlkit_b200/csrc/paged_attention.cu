@@ -224,7 +224,8 @@ template <int D> struct Shape {
   static constexpr int kTicket = kMeet + kWarps * 4;
   static constexpr int kTurns = (kTicket + 4 + 15) / 16 * 16;               // [D / 2] double: turns per position
   static constexpr int kCosine = kTurns + D / 2 * 8;                        // [D / 2][2] float
-  static constexpr int kBytes = kCosine + D / 2 * 8;
+  static constexpr int kExact = kCosine + D / 2 * 8;                        // [D / 2][2] double
+  static constexpr int kBytes = kExact + D / 2 * 16;
   static_assert(kBytes <= (kCtas == 2 ? 115712 : 232448), "shared memory");
   static_assert(kHeads * kRowFloats * 4 <= kStageBytes, "a warp's outputs fit a stage");
 };
@@ -323,6 +324,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
   const int per_row = a.kv_heads * a.head_tiles;
   double* turns_s = reinterpret_cast<double*>(smem + S::kTurns);
   float2* cosine_s = reinterpret_cast<float2*>(smem + S::kCosine);
+  double2* exact_s = reinterpret_cast<double2*>(smem + S::kExact);
   if (Rope)   // the angle in 64 bits: a far position times a frequency rounded to 32 bits is off by hundredths of a turn
     for (int i = threadIdx.x; i < D / 2; i += S::kThreads)
       turns_s[i] = exp2(-log2(double(a.theta)) * double(i) / double(D / 2)) * 0.15915494309189533577;
@@ -442,15 +444,29 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
   // where a lane's pieces lie in a stage: of the keys 32j .. and 32j + 32 .. (j even) of row g, of the values of row 2t
   const int key0 = S::key_at(g, t), key1 = S::key_at(g, t + 4), value0 = S::value_at(2 * t, g);
   int turned = -1, stage = 0;
+  bool exact = false;
   for (;;) {
     const int kv = at.head / a.head_tiles, first = (at.head - kv * a.head_tiles) * kHeads;
     const int head0 = kv * a.group + first, heads = min(kHeads, a.group - first);
-    if (Rope && turned != at.row) {
+    // The new key is turned in 64 bits: it is kept, and rounded once.  Where this run does not hold it, the queries' rotation
+    // does with 32.
+    const bool ends = Rope && at.extent.added && at.tile + count == at.extent.tiles;
+    if (Rope && (turned != at.row || (ends && !exact))) {
       turned = at.row;
+      exact = ends;
       for (int i = threadIdx.x; i < D / 2; i += S::kThreads) {
-        const double turns = double(position) * turns_s[i];
+        double turns = double(position) * turns_s[i];
+        turns -= rint(turns);
         float sine, cosine;
-        sincospif(2.f * float(turns - rint(turns)), &sine, &cosine);
+        if (ends) {
+          double2 both;
+          sincospi(2. * turns, &both.y, &both.x);
+          exact_s[i] = both;
+          cosine = float(both.x);
+          sine = float(both.y);
+        } else {
+          sincospif(2.f * float(turns), &sine, &cosine);
+        }
         cosine_s[i] = make_float2(cosine, sine);
       }
       __syncthreads();
@@ -512,7 +528,15 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
           const bool store = first == 0;
           if (lane < S::kPieces / 2) {
             float x[8], y[8];
-            rotate(new_low, new_high, 8 * lane, x, y);
+            const uint32_t l[4] = {new_low.x, new_low.y, new_low.z, new_low.w}, h[4] = {new_high.x, new_high.y, new_high.z, new_high.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 ps = Y::widen(l[e >> 1]), qs = Y::widen(h[e >> 1]);
+              const double p = e & 1 ? ps.y : ps.x, q = e & 1 ? qs.y : qs.x;
+              const double2 turn = exact_s[8 * lane + e];
+              x[e] = float(p * turn.x - q * turn.y);
+              y[e] = float(q * turn.x + p * turn.y);
+            }
             const uint4 low = make_uint4(Y::narrow(x[0], x[1]), Y::narrow(x[2], x[3]), Y::narrow(x[4], x[5]), Y::narrow(x[6], x[7]));
             const uint4 high = make_uint4(Y::narrow(y[0], y[1]), Y::narrow(y[2], y[3]), Y::narrow(y[4], y[5]), Y::narrow(y[6], y[7]));
             *reinterpret_cast<uint4*>(from + S::key_at(r, lane)) = low;

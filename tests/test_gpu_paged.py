@@ -140,11 +140,9 @@ def check_rope(lengths, positions, q_heads, kv_heads, width, page, dtype, *, slo
         q, k, v = qkv[row].view(-1, width).split((q_heads, kv_heads, kv_heads))
         id, slot = int(tables[row, n // page]), n % page
         touched[id, slot] = True
-        turned, half = rotated(k, positions[row], THETA), width // 2
-        size = k.double().abs()
-        size = size + torch.cat((size[:, half:], size[:, :half]), 1)
-        # cos and sin are off by some steps of 2^-23, a product and a sum by one each
-        assert ((k_got[id, :, slot].double() - turned).abs() <= STEP[dtype] * turned.abs() + size * 2.0 ** -21).all()
+        turned = rotated(k, positions[row], THETA)
+        # turned in 64 bits, rounded to 32 (2^-24 of the value, at most 2^-13 of half a step) and then to the cache's type
+        assert ((k_got[id, :, slot].double() - turned).abs() <= STEP[dtype] * (1 + 2.0 ** -12) * turned.abs() + 2.0 ** -25).all()
         assert torch.equal(v_got[id, :, slot], v)
         expected, bound, share, slack = attend(rotated(q, positions[row], THETA), slots_of(k_got, tables[row], n + 1),
                                                slots_of(v_got, tables[row], n + 1), width ** -0.5, dtype, True)
