@@ -63,15 +63,23 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedLayou
   };
   const bool all_held = high <= held;
   if (all_held) {
-    int p = low + threadIdx.x;
-    for (; p + 3 * kSelectThreads < high; p += 4 * kSelectThreads) {
-      uint32_t keys[4];
+    // eight at a time without a branch between them, so that their page numbers, then their weights, are under way together
+    constexpr int kDeep = 8;
+    bool missing = false;
+    for (int p = low + int(threadIdx.x); p < high; p += kDeep * kSelectThreads) {
+      int64_t at[kDeep];
+      float read[kDeep];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) keys[u] = read_key(p + u * kSelectThreads);
+      for (int u = 0; u < kDeep; ++u) at[u] = layout.weight_of(table, kv_heads, head, min(p + u * kSelectThreads, high - 1));
 #pragma unroll
-      for (int u = 0; u < 4; ++u) key_s[p + u * kSelectThreads] = keys[u];
+      for (int u = 0; u < kDeep; ++u) read[u] = __ldg(weights + max(at[u], int64_t(0)));
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        missing |= at[u] < 0;
+        if (p + u * kSelectThreads < high) key_s[p + u * kSelectThreads] = at[u] < 0 ? 0u : key_of(read[u]);
+      }
     }
-    for (; p < high; p += kSelectThreads) key_s[p] = read_key(p);
+    if (missing) atomicOr(&g_paged_evict_status, 1u);
   }
   auto key_at = [&](int p) { return all_held ? key_s[p] : read_key(p); };
   // keys over `edge` stay, and of those that equal it the first `want`
