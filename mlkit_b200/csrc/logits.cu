@@ -39,15 +39,16 @@ struct LogitArguments {
 // words meet in the first one's shared memory, since an order of (value, lower token) does not depend on who comes first.
 // Measured for 128 rows of 128256 tokens with 4000 in the history, 300 biases and a mask: penalties worked out where a piece
 // met them 115 us (almost every warp did all of it for all of its tokens), a count per token in shared memory, chunk by chunk,
-// 77 us, counts of the history's shares added into the other CTAs' memory 96 us (common tokens queued there).
+// 77 us, counts of the history's shares added into the other CTAs' memory 96 us (common tokens queued there), this form 41:
+// 15 for the copy, 5 for the mask, 14 for the history, 10 for the biases.  One row with 300 tokens of history takes 5.
 constexpr int kLogitThreads = 512;
 constexpr int kDeep = 2;                  // pieces of a thread under way
 constexpr int kSlots = 8192;              // of the hash table, at most; a power of two
-constexpr int kMost = 6144;               // tokens it takes, three quarters of its slots; more history than that goes by chunks of that many tokens
+constexpr int kMost = 6144;               // tokens it takes, three quarters of its slots; a longer history goes by chunks of a block
 constexpr int kRanks = 16;                // CTAs of a row, at most
 constexpr uint32_t kBiased = 0x80000000u; // of a count: the token has a bias
 constexpr uint32_t kSeen = 0x40000000u;   // of a count with kBiased: the token is in the history, as all without it are
-constexpr uint32_t kCount = kSeen - 1;  // how often it was generated
+constexpr uint32_t kCount = kSeen - 1;    // how often it was generated
 constexpr uint32_t kNoPlace = 0xffffffffu;
 constexpr int64_t kNothing = -(int64_t(1) << 40);
 constexpr int kBiases = 512;              // entries of a chunk that are listed in shared memory

@@ -5,11 +5,14 @@
 // What bounds it: reading the cache once, 4 * head_dim bytes a slot and key-value head for 4 * head_dim * group flops.  So:
 // * Work is cut into tiles of 16 slots of one (sequence, key-value head); the tiles of all sequences in a row are dealt out
 //   in equal runs to as many CTAs as the GPU holds, whatever the lengths.  A (sequence, head) that crosses from one CTA to
-//   the next leaves partial (max, sum, output) triples, which a second launch joins in the order of the CTAs: the
-//   workspace has two slots per CTA, independent of lengths, and there are no atomics and no state between calls.
+//   the next leaves partial (max, sum, output) triples in two slots per CTA.  Partials are joined in groups of eight CTAs,
+//   then the groups: a ticket counts the arrivals and the CTA that comes last joins, always in the order of the CTAs, so
+//   results do not depend on who that was, and leaves the ticket at zero.  (A second launch for the join measured as much on
+//   the device, 3 to 6 us, and 3 us more on the host; one level of a hundred partials 13 us.)
 // * A warp copies its own tiles into a ring of its own with cp.async, several tiles ahead, across the borders of
 //   sequences, and waits for nobody else's.  A copy instruction takes whole rows (rows cut to the 64 bytes that a lane quad
-//   feeds to the tensor core, which would spare the warp its barriers, measured 4.5 TB/s where whole ones measure 5.7).
+//   feeds to the tensor core, which would spare the warp its barriers, measured 4.5 TB/s where whole ones measure 5.7, both
+//   over the whole call).
 //   Pieces of 16 bytes are swapped within 128 bytes by the row so that neither the reads of the keys, pieces t of rows g
 //   (g = lane / 4, t = lane % 4), nor those of the values, pieces g of rows 2t, meet in a bank.  Which dimension stands at
 //   which place of a product's reduction or of its rows is free as long as queries and outputs agree, so a lane feeds the
@@ -21,6 +24,8 @@
 // * Rounding: products of 16-bit values are exact, all sums are fp32.  A softmax weight is held in two 16-bit parts (its
 //   rounding and the rest), scaled by 2^14 so that weights down to 2^-38 of the largest stay within fp16's range, and so is a
 //   rotated query: the output is rounded once, the accumulated weights are those of fp32.
+// Measured (device time, launch included): 131071 slots of 8 key-value heads of 128, 64 query heads: 94 us, 5.7 TB/s of the
+// measured 6.55; 64 sequences of 500 to 16384 slots, 32 query heads: 200 us, 6.0 TB/s; 8 sequences of 1024: 14 us.
 #include <atomic>
 
 #include "paged.cuh"

@@ -27,7 +27,7 @@ constexpr int kHeldKeys = 49152;      // keys of a sequence that lie in shared m
 // first: a histogram of the candidates that share the digits found so far says in which bin the last kept weight lies.  A
 // warp's equal digits are counted by one of its lanes: many slots have the same small weight, or one of a few exponents, and
 // queued at their bin.  Then every warp lists what it keeps of its own run of slots.  What bounds it is the chain of four
-// digits for a CTA of 16 keys a thread, 30 of the 114 us for 16 x 8 sequences of up to 16384 slots; digits of 12 and 10 bits
+// digits for a CTA of 16 keys a thread, 25 of the 110 us for 16 x 8 sequences of up to 16384 slots; digits of 12 and 10 bits
 // with the counts queueing, or with only the most common digit of a warp counted by a vote, measured no better.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedLayout layout, const float* __restrict__ weights,
                                                                       const int* __restrict__ lengths, int* __restrict__ kept,
