@@ -39,7 +39,7 @@ struct LogitArguments {
 // words meet in the first one's shared memory, since an order of (value, lower token) does not depend on who comes first.
 // Measured for 128 rows of 128256 tokens with 4000 in the history, 300 biases and a mask: penalties worked out where a piece
 // met them 115 us (almost every warp did all of it for all of its tokens), a count per token in shared memory, chunk by chunk,
-// 77 us, counts of the history's shares added into the other CTAs' memory 96 us (common tokens queued there), this form 41:
+// 77 us, counts of the history's shares added into the other CTAs' memory 96 us (common tokens queued there), this form 41 to 45:
 // 15 for the copy, 5 for the mask, 14 for the history, 10 for the biases.  One row with 300 tokens of history takes 5.
 constexpr int kLogitThreads = 512;
 constexpr int kDeep = 2;                  // pieces of a thread under way

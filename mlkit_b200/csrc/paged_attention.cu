@@ -715,7 +715,7 @@ constexpr int kWeightThreads = 256;
 template <bool Rope>
 __global__ void __launch_bounds__(kWeightThreads) paged_weight_kernel(AttentionArguments a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // lengths and tables are there: the kernel before lets this one begin only after its own wait
+  // lengths, tables and weights are there: the kernel before lets this one begin only after its own wait
   constexpr int kParts = kWeightThreads / kTile;
   const Run run = find_run<Rope, kWeightThreads>(a, a.kv_heads, kParts, blockIdx.x, gridDim.x);
   const bool idle = threadIdx.x / kTile >= run.end - run.begin;
@@ -738,11 +738,12 @@ __global__ void __launch_bounds__(kWeightThreads) paged_weight_kernel(AttentionA
     const int slot = at.tile * kTile + lane;
     const int* table = a.layout.tables + int64_t(at.row) * a.layout.table_stride;
     const int64_t to = slot < at.extent.held + at.extent.added ? a.layout.weight_of(table, a.kv_heads, at.head, slot) : -1;
+    // the slot of a new token begins at zero; the kernel before writes no weights
+    const float held = to >= 0 && slot != at.extent.held ? a.weights[to] : 0.f;
     if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
     waited = true;
     if (to >= 0) {
       float total = 0.f;
-      const float held = slot == at.extent.held ? 0.f : a.weights[to];     // the slot of a new token begins at zero
       for (int tile = 0; tile < a.head_tiles; ++tile) {
         // the scores lie in the order of the first launch: (row, head, head tile, tile)
         const int64_t from = before * a.head_tiles + (at.head * a.head_tiles + tile) * at.extent.tiles + at.tile;
