@@ -50,6 +50,7 @@ struct AttentionArguments {
   float* weights;
   int64_t q_row, q_head;    // strides in elements
   int rows, q_heads, kv_heads, group, head_tiles, ctas;
+  FastDivide by_head_tiles;
   float theta, scale_log2;
   // workspace
   float* partial;           // [ctas][2][kHeads][head_dim]: of the item a CTA's run begins within, and of the one it ends within
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
     if (page.inside) {
       const uint32_t column = a.layout.page.quotient(slot);
       page.id = uint32_t(__ldg(a.layout.tables + int64_t(ahead.row) * a.layout.table_stride + column));
-      page.inner = uint32_t(ahead.head / a.head_tiles) * a.layout.head_stride + (slot - column * a.layout.page.divisor) * a.layout.slot_stride;
+      page.inner = a.by_head_tiles.quotient(ahead.head) * a.layout.head_stride + (slot - column * a.layout.page.divisor) * a.layout.slot_stride;
     }
     return page;
   };
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
   uint32_t new_slot = kNoSlot;
   auto fetch = [&]() {
     count = min(at.extent.tiles - at.tile, run.end - done);
-    const int kv = at.head / a.head_tiles, first = (at.head - kv * a.head_tiles) * kHeads;
+    const int kv = int(a.by_head_tiles.quotient(at.head)), first = (at.head - kv * a.head_tiles) * kHeads;
     const T* source = static_cast<const T*>(a.q) + int64_t(at.row) * a.q_row;
     const uint4* q = reinterpret_cast<const uint4*>(source + int64_t(kv * a.group + first + g) * a.q_head) + t;
 #pragma unroll
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_att
   int turned = -1, stage = 0;
   bool exact = false;
   for (;;) {
-    const int kv = at.head / a.head_tiles, first = (at.head - kv * a.head_tiles) * kHeads;
+    const int kv = int(a.by_head_tiles.quotient(at.head)), first = (at.head - kv * a.head_tiles) * kHeads;
     const int head0 = kv * a.group + first, heads = min(kHeads, a.group - first);
     // The new key is turned in 64 bits: it is kept, and rounded once.  Where this run does not hold it, the queries' rotation
     // does with 32.
@@ -830,7 +831,7 @@ int attend(const char* what, AttentionArguments& a, bool rope, void* out, float*
   MKB_REQUIRE(state != nullptr && (reinterpret_cast<uintptr_t>(state) & 3) == 0, MKB_E_ARGUMENT, "%s: no state", what);
   char* base = static_cast<char*>(workspace);
   a.out = out; a.weights = weights; a.rows = M; a.q_heads = q_heads; a.kv_heads = kv_heads; a.group = q_heads / kv_heads;
-  a.head_tiles = (a.group + kHeads - 1) / kHeads; a.ctas = parts.ctas;
+  a.head_tiles = (a.group + kHeads - 1) / kHeads; a.by_head_tiles = FastDivide::of(uint32_t(a.head_tiles)); a.ctas = parts.ctas;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.partial = reinterpret_cast<float*>(base + parts.partial);
   a.partial_norm = reinterpret_cast<float2*>(base + parts.partial_norm);

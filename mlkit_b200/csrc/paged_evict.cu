@@ -28,7 +28,8 @@ constexpr int kHeldKeys = 49152;      // keys of a sequence that lie in shared m
 // warp's equal digits are counted by one of its lanes: many slots have the same small weight, or one of a few exponents, and
 // queued at their bin.  Then every warp lists what it keeps of its own run of slots.  What bounds it is the chain of four
 // digits for a CTA of 16 keys a thread, 25 of the 110 us for 16 x 8 sequences of up to 16384 slots; digits of 12 and 10 bits
-// with the counts queueing, or with only the most common digit of a warp counted by a vote, measured no better.
+// with the counts queueing, or with only the most common digit of a warp counted by a vote, measured no better, and a
+// cluster of two CTAs with half of the slots each 116.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(PagedLayout layout, const float* __restrict__ weights,
                                                                       const int* __restrict__ lengths, int* __restrict__ kept,
                                                                       int kv_heads, int budget, int sinks, int recent, int held) {
