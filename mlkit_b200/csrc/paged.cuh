@@ -34,10 +34,12 @@ struct PagedLayout {
     const uint32_t id = uint32_t(__ldg(table + column));
     return id < pages ? id * page_stride + head * head_stride + (slot - column * page.divisor) * slot_stride : kNoSlot;
   }
-  // Number of (sequence, head, slot) in an accumulator [pages, heads, page]; -1 as above.
+  // Number of (sequence, head, slot) in an accumulator [pages, heads, page]; -1 as above.  Early: before the wait for the
+  // kernel before, when the first-level cache may still hold what an earlier kernel read.
+  template <bool Early = false>
   __device__ __forceinline__ int64_t weight_of(const int* table, uint32_t heads, uint32_t head, uint32_t slot) const {
     const uint32_t column = page.quotient(slot);
-    const uint32_t id = uint32_t(__ldg(table + column));
+    const uint32_t id = uint32_t(Early ? __ldcg(table + column) : __ldg(table + column));
     return id < pages ? (int64_t(id) * heads + head) * page.divisor + (slot - column * page.divisor) : -1;
   }
   __device__ __forceinline__ int capacity() const { return int(columns * page.divisor); }

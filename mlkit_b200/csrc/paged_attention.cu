@@ -113,9 +113,9 @@ __device__ __forceinline__ uint32_t turn_matrix(uint32_t v) {   // an 8 x 8 matr
 struct Extent {
   int held, tiles, added;
 };
-template <bool Rope>
+template <bool Rope, bool Early = false>      // Early: as in PagedLayout
 __device__ __forceinline__ Extent extent_of(const AttentionArguments& a, int m, bool& beyond) {
-  const int n = __ldg(a.lengths + m), capacity = a.layout.capacity();
+  const int n = Early ? __ldcg(a.lengths + m) : __ldg(a.lengths + m), capacity = a.layout.capacity();
   if (n < 0) return {0, 0, 0};
   const int added = Rope && n < capacity;
   if (n > capacity - Rope) beyond = true;
@@ -135,7 +135,7 @@ struct Run {
     return index < longer ? index / (each + 1) : more + (index - longer) / each;
   }
 };
-template <bool Rope, int Threads>
+template <bool Rope, int Threads, bool Early = false>
 __device__ __forceinline__ Run find_run(const AttentionArguments& a, int per_row, int least, int cta, int ctas) {
   __shared__ int warp_s[Threads / 32];
   __shared__ int found_s[3];
@@ -144,7 +144,7 @@ __device__ __forceinline__ Run find_run(const AttentionArguments& a, int per_row
   const int first = min(int(threadIdx.x) * share, a.rows), last = min(first + share, a.rows);
   bool beyond = false;
   int own = 0;
-  for (int m = first; m < last; ++m) own += extent_of<Rope>(a, m, beyond).tiles;
+  for (int m = first; m < last; ++m) own += extent_of<Rope, Early>(a, m, beyond).tiles;
   if (beyond && cta == 0) atomicOr(&g_paged_attention_status, 1u);
   own *= per_row;
   int before = own;
@@ -171,7 +171,7 @@ __device__ __forceinline__ Run find_run(const AttentionArguments& a, int per_row
   if (run.begin < run.end && before <= run.begin && run.begin < before + own) {
     int rest = run.begin - before;
     for (int m = first; m < last; ++m) {
-      const Extent extent = extent_of<Rope>(a, m, beyond);
+      const Extent extent = extent_of<Rope, Early>(a, m, beyond);
       if (rest < extent.tiles * per_row) {
         found_s[0] = m;
         found_s[1] = rest / extent.tiles;
@@ -187,7 +187,7 @@ __device__ __forceinline__ Run find_run(const AttentionArguments& a, int per_row
 }
 
 // A place in the order of the tiles.
-template <bool Rope>
+template <bool Rope, bool Early = false>
 struct Cursor {
   int row, head, tile;
   Extent extent;
@@ -195,7 +195,7 @@ struct Cursor {
   // how it schedules the loop for it, measured 15 % of the whole (200 against 233 us for the ragged batch of 64).
   __device__ __forceinline__ Cursor(const AttentionArguments& a, const Run& run) : row(run.row), head(run.head), tile(run.tile) {
     bool beyond;
-    extent = extent_of<Rope>(a, row, beyond);
+    extent = extent_of<Rope, Early>(a, row, beyond);
   }
   // `steps` tiles on; the caller keeps it within the run.
   __device__ __forceinline__ void advance(const AttentionArguments& a, int per_row, int steps) {
@@ -205,7 +205,7 @@ struct Cursor {
       if (++head == per_row) {
         head = 0;
         bool beyond;
-        do extent = extent_of<Rope>(a, ++row, beyond); while (extent.tiles == 0);
+        do extent = extent_of<Rope, Early>(a, ++row, beyond); while (extent.tiles == 0);
       }
     }
   }
@@ -718,19 +718,19 @@ __global__ void __launch_bounds__(kWeightThreads) paged_weight_kernel(AttentionA
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // lengths, tables and weights are there: the kernel before lets this one begin only after its own wait
   constexpr int kParts = kWeightThreads / kTile;
-  const Run run = find_run<Rope, kWeightThreads>(a, a.kv_heads, kParts, blockIdx.x, gridDim.x);
+  const Run run = find_run<Rope, kWeightThreads, true>(a, a.kv_heads, kParts, blockIdx.x, gridDim.x);
   const bool idle = threadIdx.x / kTile >= run.end - run.begin;
   if (idle) asm volatile("griddepcontrol.wait;" ::: "memory");
   if (idle) return;
   const int part = threadIdx.x / kTile, lane = threadIdx.x % kTile, stored = min(a.group, kHeads);
-  Cursor<Rope> at(a, run);
+  Cursor<Rope, true> at(a, run);
   int before = run.begin - (at.head * at.extent.tiles + at.tile);      // tiles of the rows before
   int row = at.row;
   at.advance(a, a.kv_heads, part);
   auto catch_up = [&]() {
     for (; row < at.row; ++row) {
       bool beyond;
-      before += extent_of<Rope>(a, row, beyond).tiles * a.kv_heads;
+      before += extent_of<Rope, true>(a, row, beyond).tiles * a.kv_heads;
     }
   };
   bool waited = false;
@@ -738,9 +738,9 @@ __global__ void __launch_bounds__(kWeightThreads) paged_weight_kernel(AttentionA
     catch_up();
     const int slot = at.tile * kTile + lane;
     const int* table = a.layout.tables + int64_t(at.row) * a.layout.table_stride;
-    const int64_t to = slot < at.extent.held + at.extent.added ? a.layout.weight_of(table, a.kv_heads, at.head, slot) : -1;
+    const int64_t to = slot < at.extent.held + at.extent.added ? a.layout.weight_of<true>(table, a.kv_heads, at.head, slot) : -1;
     // the slot of a new token begins at zero; the kernel before writes no weights
-    const float held = to >= 0 && slot != at.extent.held ? a.weights[to] : 0.f;
+    const float held = to >= 0 && slot != at.extent.held ? __ldcg(a.weights + to) : 0.f;
     if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
     waited = true;
     if (to >= 0) {

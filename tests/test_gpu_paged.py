@@ -272,6 +272,35 @@ def test_results_repeat_bit_for_bit():
         assert torch.equal(out, first[0]) and torch.equal(added, first[1])
 
 
+def test_steps_in_a_row_without_waiting():
+    """Lengths, tables and queries change on the device between calls: as with a wait behind every kernel, bit for bit."""
+    results = []
+    for wait in (False, True):
+        lengths = [200, 33, 700, 5]
+        keys, values, tables, weights, _, held, _ = rope_case(lengths, lengths, 8, 2, 64, 16, HALF, seed=4)
+        wide = torch.full((4, 80), -1, dtype=torch.int32)
+        wide[:, :tables.shape[1]] = tables
+        fresh = iter(range(keys.shape[0], keys.shape[0] + 40))
+        for row in range(4):
+            for column in range(-(-(lengths[row] + 1) // 16), -(-(lengths[row] + 121) // 16)):
+                wide[row, column] = next(fresh)
+        more = lambda pool: torch.cat((pool, torch.zeros(40, *pool.shape[1:], dtype=pool.dtype))).cuda()
+        k, v, w, held, tables, shown = more(keys), more(values), more(weights), held.cuda(), torch.full_like(wide, -1).cuda(), wide.cuda()
+        generator, out = torch.Generator(device="cuda").manual_seed(0), []
+        for step in range(120):
+            qkv = torch.randn(4, 12 * 64, device="cuda", generator=generator).half()
+            tables.copy_(shown)
+            out.append(torch.empty(4, 8, 64, dtype=HALF, device="cuda"))
+            kernels.paged_rope_attention_decode(qkv, held, held, k, v, tables, out[-1], q_heads=8, kv_heads=2, head_dim=64, theta=THETA, weights=w)
+            held.add_(1)
+            if wait:
+                torch.cuda.synchronize()
+        results.append((torch.stack(out), k, v, w, held))
+    for one, other in zip(*results):
+        assert torch.equal(one.view(torch.int16) if one.dtype == HALF else one, other.view(torch.int16) if other.dtype == HALF else other)
+    assert kernels.decode_status() == 0
+
+
 def test_streams_and_graphs_that_overlap():
     """Two graphs captured on one stream and replayed on two at once, between eager calls on a third; lengths change in place."""
     cases = []
