@@ -211,10 +211,16 @@ struct Cursor {
   }
 };
 
-template <int D> struct Shape {
+// CTAs of four warps an SM.  (One CTA of eight warps for heads of 128 measured 107 us where two of four measure 91; for heads of
+// 64 without a rotation four CTAs 17 and 29 us where two measure 22 and 34, but with one, whose registers then do not
+// suffice, 43 where two with six tiles a warp measure 38; heads of 192 and 256 with more warps of two tiles each, or with two
+// CTAs of two warps, 5 to 15 % more.)
+constexpr int ctas_of(int head_dim, bool rope) { return head_dim == 64 ? (rope ? 2 : 4) : head_dim == 128 ? 2 : 1; }
+
+template <int D, bool Rope> struct Shape {
   static constexpr int kWarps = 4;
-  static constexpr int kStages = D <= 64 ? 6 : 3;
-  static constexpr int kCtas = D <= 128 ? 2 : 1;                 // per SM
+  static constexpr int kStages = D == 64 && Rope ? 6 : 3;
+  static constexpr int kCtas = ctas_of(D, Rope);                 // per SM
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kPieces = D / 8;                          // of 16 bytes in a row
   static constexpr int kOps = kTile * kPieces / 32;              // that a lane copies of the keys, and of the values
@@ -232,7 +238,7 @@ template <int D> struct Shape {
   static constexpr int kCosine = kTurns + D / 2 * 8;                        // [D / 2][2] float
   static constexpr int kExact = kCosine + D / 2 * 8;                        // [D / 2][2] double
   static constexpr int kBytes = kExact + D / 2 * 16;
-  static_assert(kBytes <= (kCtas == 2 ? 115712 : 232448), "shared memory");
+  static_assert(kBytes + 1024 <= 233472 / kCtas, "shared memory");
   static_assert(kHeads * kRowFloats * 4 <= kStageBytes, "a warp's outputs fit a stage");
 };
 
@@ -322,8 +328,8 @@ __device__ __forceinline__ bool last_of(unsigned int* ticket, int count, unsigne
 }
 
 template <typename T, int D, bool Rope>
-__global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) paged_attention_kernel(AttentionArguments a) {
-  using S = Shape<D>;
+__global__ void __launch_bounds__(Shape<D, Rope>::kThreads, Shape<D, Rope>::kCtas) paged_attention_kernel(AttentionArguments a) {
+  using S = Shape<D, Rope>;
   using Y = Types<T>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, cta = blockIdx.x;
@@ -768,7 +774,7 @@ struct Workspace {
   int ctas;
   int64_t partial, partial_norm, norm, scores, bytes;
   Workspace(int rows, int q_heads, int kv_heads, int head_dim, int page, int columns, bool weights) {
-    ctas = device_info().sm_count * (head_dim <= 128 ? 2 : 1);
+    ctas = device_info().sm_count * ctas_of(head_dim, false);
     const int group = q_heads / kv_heads, head_tiles = (group + kHeads - 1) / kHeads;
     if (ctas > MKB_PAGED_STATE_BYTES / 12) ctas = MKB_PAGED_STATE_BYTES / 12;      // three tickets each
     partial = 0;
@@ -782,7 +788,7 @@ struct Workspace {
 
 template <typename T, int D, bool Rope>
 int launch(AttentionArguments& a, void* stream) {
-  using S = Shape<D>;
+  using S = Shape<D, Rope>;
   int device = 0;
   cudaGetDevice(&device);
   static std::atomic<uint64_t> opted{0};
@@ -791,6 +797,7 @@ int launch(AttentionArguments& a, void* stream) {
     if (set != cudaSuccess) return cuda_fail(set, "paged attention shared memory");
     opted.fetch_or(uint64_t(1) << (device & 63), std::memory_order_release);
   }
+  a.ctas = min(a.ctas, device_info().sm_count * S::kCtas);
   cudaError_t launched = launch_dependent(paged_attention_kernel<T, D, Rope>, dim3(a.ctas), dim3(S::kThreads), S::kBytes, stream, a);
   if (launched == cudaSuccess && a.weights != nullptr)
     launched = launch_dependent(paged_weight_kernel<Rope>, dim3(a.ctas * 2), dim3(kWeightThreads), 0, stream, a);
