@@ -470,9 +470,13 @@ extern "C" int mkb_adjust_logits(const void* logits, void* out, const void* toke
   LogitArguments a{logits, out, history ? tokens : nullptr, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, mask,
                    static_cast<unsigned long long*>(best), static_cast<long long*>(picked), logits_stride, out_stride, tokens_stride,
                    bias_stride, mask_words, mask_stride, offset, int(width), int(history), bias ? int(biases) : 0, long_tokens, 0, 0, 0};
-  // CTAs of a row: up to sixteen, of 4096 tokens or more (one piece a thread), and two an SM in all
+  // CTAs of a row: up to sixteen, of 4096 tokens or more, and in all no more than run at once: two an SM, but a cluster of
+  // eight or sixteen lies within a group of SMs, which leaves some of its places empty (17 rows in clusters of sixteen took
+  // two turns, 15 us, in clusters of eight one, 12)
+  const int places = 2 * device_info().sm_count;
+  auto fits = [&](int64_t next) { return next <= kRanks && next / 2 * 4096 < width && next * M <= (next >= 8 ? places - 40 : places); };
   int ranks = 1;
-  while (ranks < kRanks && int64_t(ranks) * 4096 < width && int64_t(ranks) * M <= device_info().sm_count) ranks *= 2;
+  while (fits(2 * ranks)) ranks *= 2;
   // a CTA's places: as many blocks of a piece for each thread as the longest of them has; a chunk has no more tokens than the
   // table takes, unless history and biases together have no more, and then a bit map of 64 KB at most
   const int block = kLogitThreads * (dtype == MKB_F32 ? 4 : 8), blocks = int((width + 7 + block - 1) / block);
