@@ -169,9 +169,13 @@ class PagedCache:
         for row in rows:
             fresh = [self.free.pop() for _ in range(need)]
             new_tables = torch.tensor([fresh], dtype=torch.int32).to(self.device)
-            kept[row] = [kernels.evict_pages(keys, values, weights, self.tables[row:row + 1], self.lengths[row:row + 1],
-                                             new_tables, budget=budget, sinks=sinks, recent=recent)[0]
-                         for keys, values, weights in zip(self.k_pages, self.v_pages, self.weights)]
+            try:
+                kept[row] = [kernels.evict_pages(keys, values, weights, self.tables[row:row + 1], self.lengths[row:row + 1],
+                                                 new_tables, budget=budget, sinks=sinks, recent=recent)[0]
+                             for keys, values, weights in zip(self.k_pages, self.v_pages, self.weights)]
+            except Exception:
+                self.free.extend(reversed(fresh))       # the sequence stays where it was
+                raise
             self.free.extend(reversed(self.owned[row]))
             self.owned[row], self.held[row] = fresh, budget
             self.tables[row].fill_(-1)

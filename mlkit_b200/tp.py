@@ -408,6 +408,8 @@ class TensorParallelDecoder:
         batch = tokens.shape[0]
         if batch > self.max_batch:
             raise ValueError(f"batch {batch} exceeds max_batch {self.max_batch}")
+        if rules is not None and (rules.rows < batch or (rules.vocab is not None and rules.vocab < c.vocab)):
+            raise ValueError(f"rules of {rules.rows} rows and {rules.vocab} tokens for {batch} rows of {c.vocab}")
         cache, capturing = self.cache, torch.cuda.is_current_stream_capturing()
         if cache is not None:
             if not capturing:

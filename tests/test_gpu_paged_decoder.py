@@ -152,6 +152,16 @@ def test_an_eager_step_without_a_page_left_changes_nothing(parts):
     assert model.cache.held[:2] == [2, 2] and all(torch.equal(*pair) for pair in zip(before, model.cache.k_pages))
 
 
+def test_rules_that_do_not_fit_are_refused_before_the_step(parts):
+    model = build_model(CONFIG, *parts, page=8)
+    model.cache.open(0)
+    tokens, positions = torch.tensor([1, 2], device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for rules in (mk.LogitRules(rows=1, capacity=4), mk.LogitRules(rows=2, capacity=4, vocab=CONFIG.vocab - 1)):
+        with pytest.raises(ValueError, match="rules of"):
+            model.step(tokens, positions, greedy=True, rules=rules)
+    assert model.cache.held[0] == 0 and int(model.cache.lengths[0]) == 0
+
+
 def test_decoders_refuse_what_does_not_belong_together():
     with pytest.raises(ValueError, match="page size"):
         tp.TensorParallelDecoder(CONFIG, track_weights=True)

@@ -110,6 +110,19 @@ def test_prompts_are_written_behind_the_slots():
         c.write(0, 1, keys[:1], values)
 
 
+def test_an_eviction_that_fails_leaves_the_cache_as_it_was():
+    """On the CPU the kernel's wrapper refuses the pools."""
+    c = cache(track_weights=True)
+    c.open(0)
+    for _ in range(20):
+        step(c, 1)
+    before = (list(c.free), [list(pages) for pages in c.owned], list(c.held), c.tables.clone())
+    with pytest.raises(ValueError, match="CUDA"):
+        c.evict(10)
+    assert before[:3] == (c.free, c.owned, c.held) and torch.equal(before[3], c.tables)
+    consistent(c)
+
+
 def test_what_a_cache_refuses():
     for changed in ({"rows": 0}, {"columns": 0}, {"page": 0}, {"pages": 0}, {"head_dim": 96}, {"dtype": torch.float32}, {"kv_heads": 0}):
         with pytest.raises(ValueError):
