@@ -460,7 +460,11 @@ extern "C" int mkb_adjust_logits(const void* logits, void* out, const void* toke
   MKB_REQUIRE(logits && out, MKB_E_ARGUMENT, "adjust_logits: null pointer");
   MKB_REQUIRE(M == 1 || out_stride >= width, MKB_E_ARGUMENT, "adjust_logits: rows of the output overlap");
   const int64_t size = dtype_bytes(dtype);
+  // side by side in the rows of one buffer
+  const int64_t pitch = logits_stride * size, apart = int64_t(reinterpret_cast<uintptr_t>(out) - reinterpret_cast<uintptr_t>(logits));
+  const int64_t beside = pitch > 0 ? (apart % pitch + pitch) % pitch : 0;
   MKB_REQUIRE((logits == out && (M == 1 || logits_stride == out_stride)) ||
+                  (logits_stride == out_stride && beside >= width * size && pitch - beside >= width * size) ||
                   !overlap(logits, ((M - 1) * logits_stride + width) * size, out, ((M - 1) * out_stride + width) * size),
               MKB_E_ARGUMENT, "adjust_logits: the output overlaps the logits");
   MKB_REQUIRE(!tokens || history == 0 || lengths, MKB_E_ARGUMENT, "adjust_logits: a history needs its lengths");

@@ -175,3 +175,11 @@ def test_adjusted_logits_in_a_graph():
     torch.cuda.synchronize()
     expected = kernels.adjust_logits(logits, tokens=tokens, lengths=lengths, presence=presence, out=torch.empty_like(out))
     assert torch.equal(out, expected) and (out != logits).sum() > 200
+
+
+def test_logits_and_results_beside_each_other():
+    buffer = torch.randn(5, 2000, device="cuda").half()
+    expected = kernels.adjust_logits(buffer[:, :1000].contiguous(), mask=torch.full((5, 32), 0x0F0F0F0F, dtype=torch.int32, device="cuda"))
+    left = buffer[:, :1000].clone()
+    kernels.adjust_logits(buffer[:, :1000], mask=torch.full((5, 32), 0x0F0F0F0F, dtype=torch.int32, device="cuda"), out=buffer[:, 1000:])
+    assert torch.equal(buffer[:, 1000:], expected) and torch.equal(buffer[:, :1000], left)

@@ -78,6 +78,9 @@ def test_outputs_that_overlap():
     qkv = 12 * 128 * 2
     assert rope(out=POINTER, q_row=qkv // 2) == ARGUMENT and rope(out=POINTER + 2 * qkv, q_row=qkv // 2) == CUDA
     assert adjust(out=POINTER + 2000) == ARGUMENT and adjust(out=POINTER + 4000) == CUDA and adjust(out=POINTER, out_stride=1001) == ARGUMENT
+    beside = {"stride": 2100, "out_stride": 2100}      # two blocks of 1000 columns in rows of 2100
+    assert adjust(out=POINTER + 2000, **beside) == CUDA == adjust(out=POINTER - 2000, **beside) == adjust(out=POINTER + 2200, **beside)
+    assert adjust(out=POINTER + 1998, **beside) == ARGUMENT == adjust(out=POINTER + 2202, **beside) == adjust(out=POINTER - 1998, **beside)
 
 
 @needs_no_device
