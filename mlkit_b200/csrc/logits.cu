@@ -212,6 +212,15 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
         slot = (slot + 1) & (a.slots - 1);
       }
     };
+    // the history's first tokens and the first biases are under way while the table is cleared (a shard of 19 000 with biases
+    // 7.5 -> 6.9 us, eight rows of 32 bits 11.6 -> 11.3 us; a short row alone 5.3 -> 5.4 us)
+    constexpr int kEarly = 4;
+    int64_t early[kEarly];
+#pragma unroll
+    for (int u = 0; u < kEarly; ++u) early[u] = int(threadIdx.x) + u * kLogitThreads < length ? history(threadIdx.x + u * kLogitThreads) : -1;
+    const bool early_entry = int(threadIdx.x) < a.biases;
+    const int early_token = early_entry ? a.bias_tokens[m * a.bias_stride + threadIdx.x] : -1;
+    const float early_bias = early_entry ? a.bias[m * a.bias_stride + threadIdx.x] : 0.f;
     if (tracked) {
       for (int i = threadIdx.x * 4; i < 2 * a.slots + a.chunk / 32; i += kLogitThreads * 4) *reinterpret_cast<uint4*>(table_s + i) = make_uint4(0u, 0u, 0u, 0u);
       if (threadIdx.x == 0) listed_s = 0;
@@ -222,7 +231,10 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
         atomicAdd(count_s + slot_of(at), i >= prompt ? 1u : 0u);
         atomicOr(marked_s + at / 32, 1u << (at % 32));
       };
-      int i = threadIdx.x;
+#pragma unroll
+      for (int u = 0; u < kEarly; ++u)
+        if (int(threadIdx.x) + u * kLogitThreads < length) count(threadIdx.x + u * kLogitThreads, early[u]);
+      int i = threadIdx.x + kEarly * kLogitThreads;
       for (; i + 3 * kLogitThreads < length; i += 4 * kLogitThreads) {
         int64_t ids[4];
 #pragma unroll
@@ -237,7 +249,7 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
     int biases = 0;
     for (int group = 0; group < a.biases; group += kLogitThreads) {
       const int entry = group + threadIdx.x;
-      const uint32_t at = entry < a.biases ? number(a.bias_tokens[m * a.bias_stride + entry]) : kNoPlace;
+      const uint32_t at = entry < a.biases ? number(group == 0 ? early_token : a.bias_tokens[m * a.bias_stride + entry]) : kNoPlace;
       const bool inside = at != kNoPlace;
       const uint32_t votes = __ballot_sync(0xffffffffu, inside);
       if ((threadIdx.x & 31) == 0) bias_count_s[threadIdx.x >> 5] = __popc(votes);
@@ -264,7 +276,7 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
         if (slot < kBiases) {
           bias_slot_s[slot] = uint16_t(there);
           bias_at_s[slot] = int(at);
-          bias_s[slot] = a.bias[m * a.bias_stride + entry];
+          bias_s[slot] = group == 0 ? early_bias : a.bias[m * a.bias_stride + entry];
         }
       }
       __syncthreads();
