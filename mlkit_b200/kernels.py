@@ -7,6 +7,7 @@ output tensor the caller passes in, nothing is allocated.
 """
 
 import functools
+import threading
 
 import torch
 from torch import Tensor
@@ -592,42 +593,42 @@ class _AttentionScratch:
     """Where the parts of a sequence meet, on one device: a state and a workspace for each.  Calls on one stream run in order and
     share theirs; the workspace grows to the largest request.  Captured calls may be replayed at any time, so each owns its
     state for good (8 KB of a block that was cleared before) and has its workspace in the memory of its graph.  Only a call that
-    is captured when no cleared state is left has its graph clear one."""
+    is captured when no cleared state is left has its graph clear one.  The lock keeps host threads apart: a state is handed out once."""
 
     def __init__(self) -> None:
+        self.lock = threading.RLock()
         self.streams: dict[int, tuple[int, Tensor]] = {}
         self.blocks: list[Tensor] = []
         self.left: list[int] = []
 
     def refill(self, index: int) -> None:
-        self.blocks.append(torch.zeros(STATES * STATE_BYTES, dtype=torch.uint8, device=index))
+        block = torch.zeros(STATES * STATE_BYTES, dtype=torch.uint8, device=index)
         torch.cuda.current_stream(index).synchronize()        # other streams will use the states
-        self.left = [self.blocks[-1].data_ptr() + i * STATE_BYTES for i in range(STATES)] + self.left
+        self.blocks.append(block)
+        self.left = [block.data_ptr() + i * STATE_BYTES for i in range(STATES)] + self.left
 
     def of(self, index: int, stream: int, need: int) -> tuple[int, Tensor]:
-        if _capturing():
-            workspace = torch.empty(need + STATE_BYTES, dtype=torch.uint8, device=index)
-            if self.left:
-                return self.left.pop(), workspace
-            workspace[need:].zero_()
-            return workspace.data_ptr() + need, workspace
-        if len(self.left) < STATES // 2:
-            self.refill(index)
-        held = self.streams.get(stream)
-        if held is None or held[1].numel() < need:
-            held = self.streams[stream] = (self.left.pop() if held is None else held[0],
-                                           torch.empty(need, dtype=torch.uint8, device=index))
-        return held
+        with self.lock:
+            if _capturing():
+                workspace = torch.empty(need + STATE_BYTES, dtype=torch.uint8, device=index)
+                if self.left:
+                    return self.left.pop(), workspace
+                workspace[need:].zero_()
+                return workspace.data_ptr() + need, workspace
+            if len(self.left) < STATES // 2:
+                self.refill(index)
+            held = self.streams.get(stream)
+            if held is None or held[1].numel() < need:
+                held = self.streams[stream] = (self.left.pop() if held is None else held[0],
+                                               torch.empty(need, dtype=torch.uint8, device=index))
+            return held
 
 
 _attention_scratch: dict[int, _AttentionScratch] = {}
 
 
-def _scratch(index: int, stream: int, need: int) -> tuple[int, Tensor]:
-    held = _attention_scratch.get(index)
-    if held is None:
-        held = _attention_scratch[index] = _AttentionScratch()
-    return held.of(index, stream, need)
+def _scratch(index: int) -> _AttentionScratch:
+    return _attention_scratch.get(index) or _attention_scratch.setdefault(index, _AttentionScratch())
 
 
 def _check_pages(what: str, index: int, k_pages: Tensor, v_pages: Tensor, weights: Tensor | None, *tables: Tensor) -> None:
@@ -673,7 +674,7 @@ def paged_attention_decode(q: Tensor, lengths: Tensor, k_pages: Tensor, v_pages:
         with torch.cuda.device(index):
             return paged_attention_decode(q, lengths, k_pages, v_pages, tables, out, scale=scale, weights=weights)
     stream = _raw_stream(index)
-    state, workspace = _scratch(index, stream, need)
+    state, workspace = _scratch(index).of(index, stream, need)
     status = function(q.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), out.data_ptr(),
                       None if weights is None else weights.data_ptr(), *numbers, state, workspace.data_ptr(), need, stream)
     if status:
@@ -739,7 +740,7 @@ def paged_rope_attention_decode(qkv: Tensor, positions: Tensor, lengths: Tensor,
             return paged_rope_attention_decode(qkv, positions, lengths, k_pages, v_pages, tables, out, q_heads=q_heads,
                                                kv_heads=kv_heads, head_dim=head_dim, theta=theta, scale=scale, weights=weights)
     stream = _raw_stream(index)
-    state, workspace = _scratch(index, stream, need)
+    state, workspace = _scratch(index).of(index, stream, need)
     status = function(qkv.data_ptr(), positions.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                       tables.data_ptr(), out.data_ptr(), None if weights is None else weights.data_ptr(), *numbers, state,
                       workspace.data_ptr(), need, stream)

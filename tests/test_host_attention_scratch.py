@@ -1,0 +1,64 @@
+"""The states and workspaces of attention over pages, as host threads ask for them: the class on the CPU, with a stub for the
+stream it waits for."""
+
+import threading
+import time
+
+import pytest
+
+from mlkit_b200 import kernels
+
+
+class SlowStream:
+    """A stream whose wait gives the other threads their turn."""
+
+    def synchronize(self):
+        time.sleep(0.05)
+
+
+@pytest.fixture
+def on_the_cpu(monkeypatch):
+    monkeypatch.setattr(kernels.torch.cuda, "current_stream", lambda index=None: SlowStream())
+    monkeypatch.setattr(kernels, "_capturing", lambda: False)
+
+
+def in_threads(count, work):
+    """``work(i)`` in ``count`` threads that begin together; their results."""
+    results, failures, gate = [None] * count, [], threading.Barrier(count)
+
+    def run(i):
+        try:
+            gate.wait()
+            results[i] = work(i)
+        except Exception as error:
+            failures.append(error)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(count)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures
+    return results
+
+
+def test_threads_with_a_stream_each_get_states_of_their_own(on_the_cpu):
+    scratch = kernels._AttentionScratch()
+    given = in_threads(6, lambda i: scratch.of("cpu", 100 + i, 64)[0])
+    everything = given + scratch.left
+    assert len(set(everything)) == len(everything)
+    ordered = sorted(everything)
+    assert all(after - before >= kernels.STATE_BYTES for before, after in zip(ordered, ordered[1:]))
+
+
+def test_threads_that_come_first_share_one_scratch(on_the_cpu, monkeypatch):
+    monkeypatch.setattr(kernels, "_attention_scratch", {})
+    create = kernels._AttentionScratch
+
+    def slowly():
+        time.sleep(0.02)
+        return create()
+
+    monkeypatch.setattr(kernels, "_AttentionScratch", slowly)
+    given = in_threads(4, lambda i: kernels._scratch("cpu"))
+    assert all(scratch is given[0] for scratch in given)
