@@ -357,7 +357,8 @@ int mkb_argmax(const void* logits, void* best, int M, int64_t width, int64_t row
  * such slots are left out and mkb_decode_status is raised.
  * state: MKB_PAGED_STATE_BYTES bytes that are zero before the first call that uses them; every call leaves them zero.
  * workspace: mkb_paged_attention_workspace_bytes bytes (16-byte aligned), of no meaning before and after the call.
- * Calls that may run at the same time need a state and a workspace each.
+ * Calls that may run at the same time need a state and a workspace each, and so do calls that two threads make at once, on one
+ * stream too: a call with weights makes two launches, and the second reads what the first left in the workspace.
  * The reference has neither operator: it leaves attention to `transformers`.
  */
 enum { MKB_PAGED_STATE_BYTES = 8192 };

@@ -593,7 +593,9 @@ class _AttentionScratch:
     """Where the parts of a sequence meet, on one device: a state and a workspace for each.  Calls on one stream run in order and
     share theirs; the workspace grows to the largest request.  Captured calls may be replayed at any time, so each owns its
     state for good (8 KB of a block that was cleared before) and has its workspace in the memory of its graph.  Only a call that
-    is captured when no cleared state is left has its graph clear one.  The lock keeps host threads apart: a state is handed out once."""
+    is captured when no cleared state is left has its graph clear one.  The lock keeps host threads apart: a state is handed out
+    once, and callers hold it until a call's launches are all in the stream.  (A call with weights makes two, and the second
+    reads what the first left in the workspace, which threads on one stream share.)"""
 
     def __init__(self) -> None:
         self.lock = threading.RLock()
@@ -674,9 +676,11 @@ def paged_attention_decode(q: Tensor, lengths: Tensor, k_pages: Tensor, v_pages:
         with torch.cuda.device(index):
             return paged_attention_decode(q, lengths, k_pages, v_pages, tables, out, scale=scale, weights=weights)
     stream = _raw_stream(index)
-    state, workspace = _scratch(index).of(index, stream, need)
-    status = function(q.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), out.data_ptr(),
-                      None if weights is None else weights.data_ptr(), *numbers, state, workspace.data_ptr(), need, stream)
+    scratch = _scratch(index)
+    with scratch.lock:
+        state, workspace = scratch.of(index, stream, need)
+        status = function(q.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(), out.data_ptr(),
+                          None if weights is None else weights.data_ptr(), *numbers, state, workspace.data_ptr(), need, stream)
     if status:
         _native.check(status, "paged_attention_decode")
 
@@ -740,10 +744,12 @@ def paged_rope_attention_decode(qkv: Tensor, positions: Tensor, lengths: Tensor,
             return paged_rope_attention_decode(qkv, positions, lengths, k_pages, v_pages, tables, out, q_heads=q_heads,
                                                kv_heads=kv_heads, head_dim=head_dim, theta=theta, scale=scale, weights=weights)
     stream = _raw_stream(index)
-    state, workspace = _scratch(index).of(index, stream, need)
-    status = function(qkv.data_ptr(), positions.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                      tables.data_ptr(), out.data_ptr(), None if weights is None else weights.data_ptr(), *numbers, state,
-                      workspace.data_ptr(), need, stream)
+    scratch = _scratch(index)
+    with scratch.lock:
+        state, workspace = scratch.of(index, stream, need)
+        status = function(qkv.data_ptr(), positions.data_ptr(), lengths.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                          tables.data_ptr(), out.data_ptr(), None if weights is None else weights.data_ptr(), *numbers, state,
+                          workspace.data_ptr(), need, stream)
     if status:
         _native.check(status, "paged_rope_attention_decode")
 

@@ -5,6 +5,7 @@ import threading
 import time
 
 import pytest
+import torch
 
 from mlkit_b200 import kernels
 
@@ -62,3 +63,34 @@ def test_threads_that_come_first_share_one_scratch(on_the_cpu, monkeypatch):
     monkeypatch.setattr(kernels, "_AttentionScratch", slowly)
     given = in_threads(4, lambda i: kernels._scratch("cpu"))
     assert all(scratch is given[0] for scratch in given)
+
+
+@pytest.mark.parametrize("rope", [False, True])
+def test_no_call_of_another_thread_comes_between_the_launches_of_a_call(on_the_cpu, monkeypatch, rope):
+    """The C entry stands for two launches; a workspace that threads share must not be rewritten between them."""
+    monkeypatch.setattr(kernels, "_attention_scratch", {})
+    monkeypatch.setattr(kernels, "_plans", {})
+    monkeypatch.setattr(kernels, "_current_device", lambda: "cpu")
+    monkeypatch.setattr(kernels, "_raw_stream", lambda index: 7)
+    inside, overlaps = [], []
+
+    def entry(*arguments):
+        inside.append(1)
+        time.sleep(0.02)
+        overlaps.append(len(inside))
+        inside.pop()
+        return 0
+
+    monkeypatch.setattr(kernels, "_plan_rope_attention" if rope else "_plan_attention", lambda *arguments: ("cpu", entry, 64, ()))
+    rows, pages = torch.zeros(2, 4, 64), torch.zeros(3, 2, 16, 64)
+    held, tables, weights = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 1, dtype=torch.int32), torch.zeros(3, 2, 16)
+
+    def call(i):
+        if rope:
+            kernels.paged_rope_attention_decode(rows.view(2, 256), held, held, pages, pages, tables, rows, q_heads=4, kv_heads=2,
+                                                head_dim=64, theta=1e4, weights=weights)
+        else:
+            kernels.paged_attention_decode(rows, held, pages, pages, tables, rows, weights=weights)
+
+    in_threads(4, call)
+    assert overlaps == [1, 1, 1, 1]
