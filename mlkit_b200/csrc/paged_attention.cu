@@ -64,6 +64,7 @@ __device__ __forceinline__ uint32_t shared_address(const void* p) { return uint3
 
 template <typename T> struct Types;
 template <> struct Types<__half> {
+  static constexpr float kRotated = 0.5f;   // of a rotated query is held: the turn of two values of 65504 is 92637 long
   static __device__ __forceinline__ float2 widen(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
   static __device__ __forceinline__ uint32_t narrow(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
@@ -75,6 +76,7 @@ template <> struct Types<__half> {
   }
 };
 template <> struct Types<__nv_bfloat16> {
+  static constexpr float kRotated = 1.f;
   static __device__ __forceinline__ float2 widen(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   }
@@ -479,11 +481,11 @@ __global__ void __launch_bounds__(Shape<D, Rope>::kThreads, Shape<D, Rope>::kCta
         } else {
           sincospif(2.f * float(turns), &sine, &cosine);
         }
-        cosine_s[i] = make_float2(cosine, sine);
+        cosine_s[i] = make_float2(cosine * Y::kRotated, sine * Y::kRotated);
       }
       __syncthreads();
     }
-    // rotates pieces of 8 dimensions d.. and d + D/2.. of a row
+    // rotates pieces of 8 dimensions d.. and d + D/2.. of a query, times kRotated
     auto rotate = [&](const uint4& low, const uint4& high, int d, float (&x)[8], float (&y)[8]) {
       const uint32_t l[4] = {low.x, low.y, low.z, low.w}, h[4] = {high.x, high.y, high.z, high.w};
 #pragma unroll
@@ -798,6 +800,7 @@ int launch(AttentionArguments& a, void* stream) {
     opted.fetch_or(uint64_t(1) << (device & 63), std::memory_order_release);
   }
   a.ctas = min(a.ctas, device_info().sm_count * S::kCtas);
+  if (Rope) a.scale_log2 /= Types<T>::kRotated;
   cudaError_t launched = launch_dependent(paged_attention_kernel<T, D, Rope>, dim3(a.ctas), dim3(S::kThreads), S::kBytes, stream, a);
   if (launched == cudaSuccess && a.weights != nullptr)
     launched = launch_dependent(paged_weight_kernel<Rope>, dim3(a.ctas * 2), dim3(kWeightThreads), 0, stream, a);
