@@ -353,7 +353,9 @@ int mkb_argmax(const void* logits, void* best, int M, int64_t width, int64_t row
  *     sequences' tables, nor twice in one: their additions would meet.
  * head_dim 64, 128, 192 or 256; any number of query heads per key-value head.  out may be q itself, and overlaps it in no
  * other way.  What lies in slots behind a sequence's length is never used; queries, keys and values in use are finite (an
- * infinity may give NaN where it need not: weights and rotated queries are held as two 16-bit parts).  A length beyond the table, and an entry that is no page of the pool, never become an address:
+ * infinity may give NaN where it need not: weights and rotated queries are held as 16-bit parts).  Two parts leave out, in
+ * fp16 and bf16, 2^-22 and 2^-17 of a softmax weight in the output, and of a score 2^-23 and 2^-17 of scale * sum |q k| after a
+ * rotation; with accumulated weights a rotated bf16 query has a third part, and scores are those of fp32.  A length beyond the table, and an entry that is no page of the pool, never become an address:
  * such slots are left out and mkb_decode_status is raised.
  * state: MKB_PAGED_STATE_BYTES bytes that are zero before the first call that uses them; every call leaves them zero.
  * workspace: mkb_paged_attention_workspace_bytes bytes (16-byte aligned), of no meaning before and after the call.

@@ -22,8 +22,11 @@
 //   layout to the operand's with movmatrix.  More than eight heads of a group are several tiles of heads, which read the
 //   cache again (from L2, mostly).
 // * Rounding: products of 16-bit values are exact, all sums are fp32.  A softmax weight is held in two 16-bit parts (its
-//   rounding and the rest), scaled by 2^14 so that weights down to 2^-38 of the largest stay within fp16's range, and so is a
-//   rotated query: the output is rounded once, the accumulated weights are those of fp32.
+//   rounding and the rest) for the product with the values, scaled by 2^14 so that weights down to 2^-38 of the largest stay
+//   within fp16's range: 2^-22 of it is left out in fp16 and 2^-17 in bf16, far below the step the output is rounded to.  So is a
+//   rotated query: 2^-23 of a value (2^-24 absolute for small ones) in fp16, 2^-17 in bf16, of which a score is off by as much of
+//   sum |q k|.  Weights that are accumulated are taken from the scores in fp32; for them a bf16 query has a third part, which
+//   leaves out less than fp32 does.
 // Measured (device time, launch included): 131071 slots of 8 key-value heads of 128, 64 query heads: 94 us, 5.7 TB/s of the
 // measured 6.55; 64 sequences of 500 to 16384 slots, 32 query heads: 200 us, 6.0 TB/s; 8 sequences of 1024: 14 us.
 #include <atomic>
@@ -219,7 +222,7 @@ struct Cursor {
 // CTAs of two warps, 5 to 15 % more.)
 constexpr int ctas_of(int head_dim, bool rope) { return head_dim == 64 ? (rope ? 2 : 4) : head_dim == 128 ? 2 : 1; }
 
-template <int D, bool Rope> struct Shape {
+template <int D, bool Rope, bool Weighted> struct Shape {
   static constexpr int kWarps = 4;
   static constexpr int kStages = D == 64 && Rope ? 6 : 3;
   static constexpr int kCtas = ctas_of(D, Rope);                 // per SM
@@ -239,7 +242,8 @@ template <int D, bool Rope> struct Shape {
   static constexpr int kTurns = (kTicket + 4 + 15) / 16 * 16;               // [D / 2] double: turns per position
   static constexpr int kCosine = kTurns + D / 2 * 8;                        // [D / 2][2] float
   static constexpr int kExact = kCosine + D / 2 * 8;                        // [D / 2][2] double
-  static constexpr int kBytes = kExact + D / 2 * 16;
+  static constexpr int kThird = kExact + D / 2 * 16;                        // [warp][D / 32][lane] uint4: third parts of rotated queries
+  static constexpr int kBytes = kThird + (Weighted ? kWarps * D * 16 : 0);
   static_assert(kBytes + 1024 <= 233472 / kCtas, "shared memory");
   static_assert(kHeads * kRowFloats * 4 <= kStageBytes, "a warp's outputs fit a stage");
 };
@@ -329,9 +333,12 @@ __device__ __forceinline__ bool last_of(unsigned int* ticket, int count, unsigne
   return *shared == unsigned(count - 1);
 }
 
-template <typename T, int D, bool Rope>
-__global__ void __launch_bounds__(Shape<D, Rope>::kThreads, Shape<D, Rope>::kCtas) paged_attention_kernel(AttentionArguments a) {
-  using S = Shape<D, Rope>;
+// Weighted: weights are accumulated, for which rotated bf16 queries are held in a third part.  Of no use to the output, which is
+// rounded to 2^-8, and not free: eight sequences of 1024, 32 query heads of 128: 14.7 us where two parts take 13.9, of 3000
+// to 6000, heads of 192: 50 and 44, of 256: 61 and 55 (the ragged batch of 64 measured no difference).
+template <typename T, int D, bool Rope, bool Weighted>
+__global__ void __launch_bounds__(Shape<D, Rope, Weighted>::kThreads, Shape<D, Rope, Weighted>::kCtas) paged_attention_kernel(AttentionArguments a) {
+  using S = Shape<D, Rope, Weighted>;
   using Y = Types<T>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, cta = blockIdx.x;
@@ -499,6 +506,7 @@ __global__ void __launch_bounds__(Shape<D, Rope>::kThreads, Shape<D, Rope>::kCta
     };
     // queries: head g, dimensions 32j + 8t ..
     uint32_t query[D / 32][4], rest[Rope ? D / 32 : 1][4];
+    uint4* third_s = reinterpret_cast<uint4*>(smem + S::kThird) + warp * D + lane;
     {
       if constexpr (Rope) {
 #pragma unroll
@@ -509,6 +517,17 @@ __global__ void __launch_bounds__(Shape<D, Rope>::kThreads, Shape<D, Rope>::kCta
           for (int i = 0; i < 4; ++i) {
             split<T>(x[2 * i], x[2 * i + 1], query[j][i], rest[j][i]);
             split<T>(y[2 * i], y[2 * i + 1], query[j + D / 64][i], rest[j + D / 64][i]);
+          }
+          if constexpr (Weighted) {
+            auto left = [](uint32_t pair, uint32_t rest, float lo, float hi) {
+              const float2 a = Y::widen(pair), b = Y::widen(rest);
+              return Y::narrow(lo - a.x - b.x, hi - a.y - b.y);
+            };
+            const int k = j + D / 64;
+            third_s[j * 32] = make_uint4(left(query[j][0], rest[j][0], x[0], x[1]), left(query[j][1], rest[j][1], x[2], x[3]),
+                                         left(query[j][2], rest[j][2], x[4], x[5]), left(query[j][3], rest[j][3], x[6], x[7]));
+            third_s[k * 32] = make_uint4(left(query[k][0], rest[k][0], y[0], y[1]), left(query[k][1], rest[k][1], y[2], y[3]),
+                                         left(query[k][2], rest[k][2], y[4], y[5]), left(query[k][3], rest[k][3], y[6], y[7]));
           }
         }
       } else {
@@ -579,6 +598,11 @@ __global__ void __launch_bounds__(Shape<D, Rope>::kThreads, Shape<D, Rope>::kCta
         if constexpr (Rope) {
           Y::mma(small, x.x, y.x, x.y, y.y, rest[j][0], rest[j][1]);
           Y::mma(small, x.z, y.z, x.w, y.w, rest[j][2], rest[j][3]);
+          if constexpr (Weighted) {
+            const uint4 third = third_s[j * 32];
+            Y::mma(small, x.x, y.x, x.y, y.y, third.x, third.y);
+            Y::mma(small, x.z, y.z, x.w, y.w, third.z, third.w);
+          }
         }
       }
 #pragma unroll
@@ -788,33 +812,33 @@ struct Workspace {
   }
 };
 
-template <typename T, int D, bool Rope>
+template <typename T, int D, bool Rope, bool Weighted>
 int launch(AttentionArguments& a, void* stream) {
-  using S = Shape<D, Rope>;
+  using S = Shape<D, Rope, Weighted>;
   int device = 0;
   cudaGetDevice(&device);
   static std::atomic<uint64_t> opted{0};
   if (!(opted.load(std::memory_order_acquire) >> (device & 63) & 1)) {
-    const cudaError_t set = cudaFuncSetAttribute(paged_attention_kernel<T, D, Rope>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    const cudaError_t set = cudaFuncSetAttribute(paged_attention_kernel<T, D, Rope, Weighted>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
     if (set != cudaSuccess) return cuda_fail(set, "paged attention shared memory");
     opted.fetch_or(uint64_t(1) << (device & 63), std::memory_order_release);
   }
   a.ctas = min(a.ctas, device_info().sm_count * S::kCtas);
   if (Rope) a.scale_log2 /= Types<T>::kRotated;
-  cudaError_t launched = launch_dependent(paged_attention_kernel<T, D, Rope>, dim3(a.ctas), dim3(S::kThreads), S::kBytes, stream, a);
+  cudaError_t launched = launch_dependent(paged_attention_kernel<T, D, Rope, Weighted>, dim3(a.ctas), dim3(S::kThreads), S::kBytes, stream, a);
   if (launched == cudaSuccess && a.weights != nullptr)
     launched = launch_dependent(paged_weight_kernel<Rope>, dim3(a.ctas * 2), dim3(kWeightThreads), 0, stream, a);
   if (launched != cudaSuccess) return cuda_fail(launched, "paged attention launch");
   return MKB_OK;
 }
 
-template <typename T, bool Rope>
+template <typename T, bool Rope, bool Weighted = false>
 int dispatch(AttentionArguments& a, int head_dim, void* stream) {
   switch (head_dim) {
-    case 64: return launch<T, 64, Rope>(a, stream);
-    case 128: return launch<T, 128, Rope>(a, stream);
-    case 192: return launch<T, 192, Rope>(a, stream);
-    default: return launch<T, 256, Rope>(a, stream);
+    case 64: return launch<T, 64, Rope, Weighted>(a, stream);
+    case 128: return launch<T, 128, Rope, Weighted>(a, stream);
+    case 192: return launch<T, 192, Rope, Weighted>(a, stream);
+    default: return launch<T, 256, Rope, Weighted>(a, stream);
   }
 }
 
@@ -849,6 +873,7 @@ int attend(const char* what, AttentionArguments& a, bool rope, void* out, float*
   a.norm = reinterpret_cast<float*>(base + parts.norm);
   a.scores = reinterpret_cast<float*>(base + parts.scores);
   if (dtype == MKB_F16) return rope ? dispatch<__half, true>(a, head_dim, stream) : dispatch<__half, false>(a, head_dim, stream);
+  if (rope && weights != nullptr) return dispatch<__nv_bfloat16, true, true>(a, head_dim, stream);
   return rope ? dispatch<__nv_bfloat16, true>(a, head_dim, stream) : dispatch<__nv_bfloat16, false>(a, head_dim, stream);
 }
 
