@@ -27,12 +27,12 @@ struct LogitArguments {
   unsigned long long* best;
   long long* picked;
   int64_t logits_stride, out_stride, tokens_stride, bias_stride, mask_words, mask_stride, offset;
-  int width, history, biases, long_tokens, slice, chunk, slots;
+  int width, history, biases, long_tokens, slice, widest, slots;    // widest: tokens of the longest chunk
 };
 
 // What bounds it: for many rows the logits, read and written once (4 bytes a token in 16 bits); for few, the chain of
 // launch, history and one reduction.  So a row is spread over a cluster of CTAs, as many as keep the GPU busy, each with a
-// slice of the vocabulary.  A CTA reads the whole history once, gathers the slice's tokens with their counts in a hash table
+// slice of the vocabulary.  A CTA reads the whole history, gathers the slice's tokens with their counts in a hash table
 // in shared memory (no [rows, vocabulary] state exists anywhere) and marks them in a bit map, while its first logits are
 // under way.  Then the slice passes in 16-byte pieces as it is, masked in its own type, but for the marked tokens, and the
 // greedy pick looks at a piece's maximum only; the marked tokens follow from the table's list, one a thread.  The CTAs' best
@@ -124,13 +124,13 @@ __device__ __forceinline__ unsigned long long word_of(uint32_t key, uint32_t tok
 template <typename T>
 __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitArguments a) {
   using L = Logit<T>;
-  constexpr int V = L::kVector;
+  constexpr int V = L::kVector, kBlock = kLogitThreads * V;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // every CTA runs before another writes to it
   extern __shared__ __align__(16) uint32_t table_s[];   // with a history or biases: keys, counts, bit map, list of slots
   uint32_t* count_s = table_s + a.slots;
   uint32_t* marked_s = count_s + a.slots;
-  uint16_t* list_s = reinterpret_cast<uint16_t*>(marked_s + a.chunk / 32);
+  uint16_t* list_s = reinterpret_cast<uint16_t*>(marked_s + a.widest / 32);
   __shared__ int bias_at_s[kBiases], bias_count_s[kLogitThreads / 32], listed_s;
   __shared__ float bias_s[kBiases];
   __shared__ uint16_t bias_slot_s[kBiases];
@@ -154,10 +154,16 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
   const float frequency = a.frequency ? a.frequency[m] : 0.f, presence = a.presence ? a.presence[m] : 0.f;
   const uint32_t* mask = reinterpret_cast<const uint32_t*>(a.mask) + m * a.mask_stride;
   const bool tracked = length > 0 || a.biases > 0;
+  // Chunks go by the row's own text, whatever the width of its buffer: the whole slice at a time when the table takes all that the row
+  // notes, else a block, which has no more tokens than the table takes, with the history read again for each.  (Rows of 300 tokens
+  // in a buffer of 32768, chunks by the width of the buffer and by the text: one row 12.8 and 9.0 us, 128 rows 97 and 25, in a
+  // buffer of 300 8.2 and 25.  A table of the text's size as well takes 0.5 us off one such row and adds 1 us to 128 rows with texts of
+  // 4000.  Texts of 30000: one row 42, 128 rows 373 us.)
+  const int noted = length + a.biases;
+  const int chunk = noted <= kMost ? a.widest : kBlock;
 
   // the row's blocks of a piece for each thread go to the CTAs in turn, so that common tokens, which lie together, do not
   // meet in one; a CTA numbers its own places through
-  constexpr int kBlock = kLogitThreads * V;
   const int end = a.width + shift, turn = __ffs(ranks) - 1;
   auto place_of = [&](int local) { return ((local / kBlock << turn) + int(rank)) * kBlock + local % kBlock; };
   unsigned long long top = 0;                  // of what the list takes
@@ -176,8 +182,8 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
         asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row + from), "r"(uint32_t((to - from) * sizeof(T))) : "memory");
     }
   }
-  for (int base = 0;; base += a.chunk) {
-    const int last = min(base + a.chunk, a.slice);
+  for (int base = 0;; base += chunk) {
+    const int last = min(base + chunk, a.slice);
     // the chunk's first logits, and their bits of the mask
     uint4 held[kDeep];
     uint64_t bits[kDeep];
@@ -222,7 +228,7 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
     const int early_token = early_entry ? a.bias_tokens[m * a.bias_stride + threadIdx.x] : -1;
     const float early_bias = early_entry ? a.bias[m * a.bias_stride + threadIdx.x] : 0.f;
     if (tracked) {
-      for (int i = threadIdx.x * 4; i < 2 * a.slots + a.chunk / 32; i += kLogitThreads * 4) *reinterpret_cast<uint4*>(table_s + i) = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = threadIdx.x * 4; i < 2 * a.slots + a.widest / 32; i += kLogitThreads * 4) *reinterpret_cast<uint4*>(table_s + i) = make_uint4(0u, 0u, 0u, 0u);
       if (threadIdx.x == 0) listed_s = 0;
       __syncthreads();
       auto count = [&](int i, int64_t id) {
@@ -429,7 +435,7 @@ int launch_logits(const LogitArguments& a, int M, int ranks, void* stream) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(ranks, M);
   config.blockDim = dim3(kLogitThreads);
-  config.dynamicSmemBytes = a.tokens || a.bias ? a.slots * 8 + a.slots * 3 / 4 * 2 + a.chunk / 8 : 0;
+  config.dynamicSmemBytes = a.tokens || a.bias ? a.slots * 8 + a.slots * 3 / 4 * 2 + a.widest / 8 : 0;
   int device = 0;
   cudaGetDevice(&device);
   static std::atomic<uint64_t> opted{0};
@@ -493,12 +499,12 @@ extern "C" int mkb_adjust_logits(const void* logits, void* out, const void* toke
   auto fits = [&](int64_t next) { return next <= kRanks && next / 2 * 4096 < width && next * M <= (next >= 8 ? places - 40 : places); };
   int ranks = 1;
   while (fits(2 * ranks)) ranks *= 2;
-  // a CTA's places: as many blocks of a piece for each thread as the longest of them has; a chunk has no more tokens than the
-  // table takes, unless history and biases together have no more, and then a bit map of 64 KB at most
+  // a CTA's places: as many blocks of a piece for each thread as the longest of them has; the bit map of a chunk has 64 KB at
+  // most, and the table room for what the widest text that fits the buffer needs
   const int block = kLogitThreads * (dtype == MKB_F32 ? 4 : 8), blocks = int((width + 7 + block - 1) / block);
   a.slice = (blocks + ranks - 1) / ranks * block;
   const int64_t noted = (a.tokens ? history : 0) + a.biases;
-  a.chunk = noted <= kMost ? (a.slice < 1 << 19 ? a.slice : 1 << 19) : block;
+  a.widest = a.slice < 1 << 19 ? a.slice : 1 << 19;
   a.slots = kLogitThreads;
   while (a.slots < kSlots && a.slots * 3 / 4 < noted) a.slots *= 2;
   static_assert(kMost == kSlots * 3 / 4, "the table's size");
