@@ -247,6 +247,15 @@ class LogitRules:
         history.scatter_(1, at, torch.where(room.unsqueeze(1), tokens.unsqueeze(1), history.gather(1, at)))
         self.lengths[:batch].add_(room)
 
+    @contextmanager
+    def idle(self) -> Iterator[None]:
+        """What is observed meanwhile is not kept: steps that warm up or are captured leave the histories as they are."""
+        saved = self.lengths.clone()
+        try:
+            yield
+        finally:
+            self.lengths.copy_(saved)
+
     def apply(self, logits: Tensor, *, offset: int = 0, best: Tensor | None = None, picked: Tensor | None = None) -> Tensor:
         """``logits`` [batch, width] of the tokens ``offset..offset + width``, adjusted in place by the first ``batch`` rows' rules."""
         batch = logits.shape[0]

@@ -506,20 +506,19 @@ class CapturedStep:
         self.model, self.batch = model, batch
         self.tokens = torch.zeros(batch, dtype=torch.int64, device=model.device)
         self.positions = torch.zeros(batch, dtype=torch.int32, device=model.device)
-        with model.cache.idle() if model.cache is not None else nullcontext():
-            observed = None if rules is None else rules.lengths.clone()
+        with model.cache.idle() if model.cache is not None else nullcontext(), rules.idle() if rules is not None else nullcontext():
             side = torch.cuda.Stream(device=model.device)
             side.wait_stream(torch.cuda.current_stream(model.device))
-            with torch.cuda.stream(side):
-                for _ in range(2):  # warm up kernels, NCCL channels and the allocator before capturing
-                    model.step(self.tokens, self.positions, greedy, rules)
-                torch.cuda.synchronize(model.device)
-                self.graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(self.graph, stream=side):
-                    self.logits = model.step(self.tokens, self.positions, greedy, rules)
-            torch.cuda.current_stream(model.device).wait_stream(side)
-            if rules is not None:
-                rules.lengths.copy_(observed)
+            try:
+                with torch.cuda.stream(side):
+                    for _ in range(2):  # warm up kernels, NCCL channels and the allocator before capturing
+                        model.step(self.tokens, self.positions, greedy, rules)
+                    torch.cuda.synchronize(model.device)
+                    self.graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(self.graph, stream=side):
+                        self.logits = model.step(self.tokens, self.positions, greedy, rules)
+            finally:   # when a step fails as well: what the steps counted is taken back behind them
+                torch.cuda.current_stream(model.device).wait_stream(side)
         torch.cuda.synchronize(model.device)
 
     def replay(self) -> Tensor:
