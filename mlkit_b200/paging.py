@@ -27,7 +27,9 @@ class PagedCache:
     slot's attention weight is added up, and ``evict`` can cut sequences down to a budget of slots.
 
     The bookkeeping is on the host (``held`` mirrors ``lengths``): a step calls ``prepare`` before its launches and ``advance``
-    after them, of which only the addition to ``lengths`` is device work, so captured steps replay without synchronising.
+    after them.  On the device that is the addition to ``lengths`` and, when sequences begin pages, one copy of their numbers from
+    pinned memory into ``tables``, so captured steps replay without synchronising; opening, releasing and evicting do not wait
+    either.
     """
 
     def __init__(self, *, rows: int, columns: int, kv_heads: int, head_dim: int, page: int = 16, pages: int | None = None,
@@ -73,13 +75,13 @@ class PagedCache:
         if self.held[row] >= 0:
             raise ValueError(f"row {row} is in use")
         self.held[row] = 0
-        self.lengths[row] = 0
+        self.lengths[row].fill_(0)
 
     def release(self, row: int) -> None:
         """End a row's sequence, if it has one, and give its pages back."""
         self.free.extend(reversed(self.owned[row]))
         self.owned[row], self.held[row] = [], -1
-        self.lengths[row] = -1
+        self.lengths[row].fill_(-1)
 
     def reserve(self, row: int, slots: int) -> None:
         """Take the pages that ``slots`` slots of the row's sequence need, all of them or, with an error, none."""
@@ -93,13 +95,25 @@ class PagedCache:
             if slots > self.capacity:
                 raise ValueError(f"a sequence of {slots} slots exceeds the {self.columns} pages of {self.page} of a row")
             counts.append((row, max(0, -(-slots // self.page) - len(self.owned[row]))))
-        if sum(count for _, count in counts) > len(self.free):
-            raise RuntimeError(f"the cache has {len(self.free)} free pages, {sum(count for _, count in counts)} are needed")
+        total = sum(count for _, count in counts)
+        if total > len(self.free):
+            raise RuntimeError(f"the cache has {len(self.free)} free pages, {total} are needed")
+        if not total:
+            return
+        pages = self.free[:-total - 1:-1]
+        places = [row % self.rows * self.columns + len(self.owned[row]) + i for row, count in counts for i in range(count)]
+        sent = self._sent([places, pages])
+        self.tables.view(-1).index_copy_(0, sent[0], sent[1].int())
+        del self.free[-total:]
         for row, count in counts:
-            if count:
-                start = len(self.owned[row])
-                self.owned[row].extend(self.free.pop() for _ in range(count))
-                self.tables[row, start:start + count] = torch.tensor(self.owned[row][start:], dtype=torch.int32)
+            self.owned[row].extend(pages[:count])
+            del pages[:count]
+
+    def _sent(self, numbers: list[list[int]]) -> Tensor:
+        """``numbers`` on the device, in stream order.  A copy from memory that is not pinned would wait for the stream, as would
+        assigning a number to an element, for which this class has ``fill_``."""
+        given = torch.tensor(numbers, dtype=torch.int64)
+        return given.pin_memory().to(self.device, non_blocking=True) if self.device.type == "cuda" else given
 
     def write(self, layer: int, row: int, keys: Tensor, values: Tensor) -> None:
         """Put a prompt's rotated keys and its values, [kv_heads, tokens, head_dim], behind the row's slots in one layer; call
@@ -120,7 +134,7 @@ class PagedCache:
         """Count ``tokens`` slots that ``write`` has filled."""
         self.reserve(row, self.held[row] + tokens)
         self.held[row] += tokens
-        self.lengths[row] = self.held[row]
+        self.lengths[row].fill_(self.held[row])
 
     # -- steps --
     def prepare(self, batch: int) -> None:
@@ -168,7 +182,7 @@ class PagedCache:
             raise RuntimeError(f"the cache has {len(self.free)} free pages, {need} are needed to evict into")
         for row in rows:
             fresh = [self.free.pop() for _ in range(need)]
-            new_tables = torch.tensor([fresh], dtype=torch.int32).to(self.device)
+            new_tables = self._sent([fresh]).int()
             try:
                 kept[row] = [kernels.evict_pages(keys, values, weights, self.tables[row:row + 1], self.lengths[row:row + 1],
                                                  new_tables, budget=budget, sinks=sinks, recent=recent)[0]
@@ -180,7 +194,7 @@ class PagedCache:
             self.owned[row], self.held[row] = fresh, budget
             self.tables[row].fill_(-1)
             self.tables[row, :need] = new_tables[0]
-            self.lengths[row] = budget
+            self.lengths[row].fill_(budget)
         return kept
 
 
