@@ -592,10 +592,11 @@ STATE_BYTES, STATES = 8192, 128     # of the attention over pages: zeroed words 
 class _AttentionScratch:
     """Where the parts of a sequence meet, on one device: a state and a workspace for each.  Calls on one stream run in order and
     share theirs; the workspace grows to the largest request.  Captured calls may be replayed at any time, so each owns its
-    state for good (8 KB of a block that was cleared before) and has its workspace in the memory of its graph.  Only a call that
-    is captured when no cleared state is left has its graph clear one.  The lock keeps host threads apart: a state is handed out
-    once, and callers hold it until a call's launches are all in the stream.  (A call with weights makes two, and the second
-    reads what the first left in the workspace, which threads on one stream share.)"""
+    state for good, also when its graph is gone (8 KB of a block that was cleared before), and has its workspace in the memory of its
+    graph.  After every eager call there are STATES for the captures to come; only a call that is captured when none is left has its
+    graph clear one.  The lock keeps host threads apart: a state is handed out once, and callers hold it until a call's launches are
+    all in the stream.  (A call with weights makes two, and the second reads what the first left in the workspace, which threads
+    on one stream share.)"""
 
     def __init__(self) -> None:
         self.lock = threading.RLock()
@@ -617,7 +618,7 @@ class _AttentionScratch:
                     return self.left.pop(), workspace
                 workspace[need:].zero_()
                 return workspace.data_ptr() + need, workspace
-            if len(self.left) < STATES // 2:
+            while len(self.left) < STATES + (stream not in self.streams):     # so that STATES are left
                 self.refill(index)
             held = self.streams.get(stream)
             if held is None or held[1].numel() < need:

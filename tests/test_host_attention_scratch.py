@@ -94,3 +94,15 @@ def test_no_call_of_another_thread_comes_between_the_launches_of_a_call(on_the_c
 
     in_threads(4, call)
     assert overlaps == [1, 1, 1, 1]
+
+
+def test_after_an_eager_call_there_are_states_for_a_whole_capture(on_the_cpu, monkeypatch):
+    scratch = kernels._AttentionScratch()
+    for attempt in range(5):
+        scratch.of("cpu", 7 + attempt, 64)
+        assert len(scratch.left) >= kernels.STATES
+        monkeypatch.setattr(kernels, "_capturing", lambda: True)
+        given = [scratch.of("cpu", 7, 64)[0] for _ in range(100)]
+        monkeypatch.setattr(kernels, "_capturing", lambda: False)
+        blocks = [(block.data_ptr(), block.data_ptr() + block.numel()) for block in scratch.blocks]
+        assert all(any(low <= state < high for low, high in blocks) for state in given)      # none is its graph's to clear
