@@ -430,12 +430,11 @@ __global__ void __launch_bounds__(kLogitThreads, 2) adjust_logits_kernel(LogitAr
   }
 }
 
+// Dynamic shared memory of a launch with tables of `slots` and chunks of up to `widest` tokens.
+size_t table_bytes(int slots, int widest) { return size_t(slots) * 8 + slots * 3 / 4 * 2 + widest / 8; }
+
 template <typename T>
-int launch_logits(const LogitArguments& a, int M, int ranks, void* stream) {
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(ranks, M);
-  config.blockDim = dim3(kLogitThreads);
-  config.dynamicSmemBytes = a.tokens || a.bias ? a.slots * 8 + a.slots * 3 / 4 * 2 + a.widest / 8 : 0;
+int launch_logits(LogitArguments& a, int M, void* stream) {
   int device = 0;
   cudaGetDevice(&device);
   static std::atomic<uint64_t> opted{0};
@@ -445,14 +444,45 @@ int launch_logits(const LogitArguments& a, int M, int ranks, void* stream) {
     if (set != cudaSuccess) return cuda_fail(set, "adjust_logits attributes");
     opted.fetch_or(uint64_t(1) << (device & 63), std::memory_order_release);
   }
+  cudaLaunchConfig_t config{};
+  config.blockDim = dim3(kLogitThreads);
   config.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attribute[2];
-  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute[0].val.programmaticStreamSerializationAllowed = 1;
-  attribute[1].id = cudaLaunchAttributeClusterDimension;
-  attribute[1].val.clusterDim.x = ranks;
-  attribute[1].val.clusterDim.y = attribute[1].val.clusterDim.z = 1;
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+  attribute[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
+  constexpr int kBlock = kLogitThreads * Logit<T>::kVector;
+  const bool tracked = a.tokens || a.bias;
+  // a CTA's places: as many blocks of a piece for each thread as the longest of them has; the bit map of a chunk has 64 KB at
+  // most, and the table room for what the widest text that fits the buffer needs
+  auto shape = [&](int ranks) {
+    const int blocks = (a.width + 7 + kBlock - 1) / kBlock;
+    a.slice = (blocks + ranks - 1) / ranks * kBlock;
+    a.widest = a.slice < 1 << 19 ? a.slice : 1 << 19;
+    config.gridDim = dim3(ranks, M);
+    config.dynamicSmemBytes = tracked ? table_bytes(a.slots, a.widest) : 0;
+    attribute[0].val.clusterDim.x = ranks;
+  };
+  // CTAs of a row: up to sixteen, of 4096 tokens or more, and in all no more than run at once, which for clusters is less than
+  // for CTAs, since a cluster lies within a group of SMs (of sixteen 14 run at once, 224 of 296 CTAs): 16 rows of 50257 in 32 bits
+  // took two turns of clusters of sixteen, 15 us, and take one of clusters of eight, 11.  The answer for the last call's sizes is kept: asking the runtime takes some microseconds.
+  thread_local struct { int device, rows, width, slots; bool tracked; int ranks; } last{-1, 0, 0, 0, false, 0};
+  if (last.device != device || last.rows != M || last.width != a.width || last.slots != a.slots || last.tracked != tracked) {
+    int ranks = 1;
+    for (int next = 2; next <= kRanks && next / 2 * 4096 < a.width; next *= 2) {
+      shape(next);
+      config.numAttrs = 1;
+      int clusters = 0;
+      const cudaError_t asked = cudaOccupancyMaxActiveClusters(&clusters, adjust_logits_kernel<T>, &config);
+      if (asked != cudaSuccess) return cuda_fail(asked, "adjust_logits clusters");
+      if (clusters < M) break;
+      ranks = next;
+    }
+    last = {device, M, a.width, a.slots, tracked, ranks};
+  }
+  shape(last.ranks);
   config.numAttrs = 2;
   const cudaError_t launched = cudaLaunchKernelEx(&config, adjust_logits_kernel<T>, a);
   if (launched != cudaSuccess) return cuda_fail(launched, "adjust_logits launch");
@@ -492,27 +522,15 @@ extern "C" int mkb_adjust_logits(const void* logits, void* out, const void* toke
   LogitArguments a{logits, out, history ? tokens : nullptr, lengths, prompts, repetition, frequency, presence, bias_tokens, bias, mask,
                    static_cast<unsigned long long*>(best), static_cast<long long*>(picked), logits_stride, out_stride, tokens_stride,
                    bias_stride, mask_words, mask_stride, offset, int(width), int(history), bias ? int(biases) : 0, long_tokens, 0, 0, 0};
-  // CTAs of a row: up to sixteen, of 4096 tokens or more, and in all no more than run at once: two an SM, but a cluster of
-  // eight or sixteen lies within a group of SMs, which leaves some of its places empty (17 rows in clusters of sixteen took
-  // two turns, 15 us, in clusters of eight one, 12)
-  const int places = 2 * device_info().sm_count;
-  auto fits = [&](int64_t next) { return next <= kRanks && next / 2 * 4096 < width && next * M <= (next >= 8 ? places - 40 : places); };
-  int ranks = 1;
-  while (fits(2 * ranks)) ranks *= 2;
-  // a CTA's places: as many blocks of a piece for each thread as the longest of them has; the bit map of a chunk has 64 KB at
-  // most, and the table room for what the widest text that fits the buffer needs
-  const int block = kLogitThreads * (dtype == MKB_F32 ? 4 : 8), blocks = int((width + 7 + block - 1) / block);
-  a.slice = (blocks + ranks - 1) / ranks * block;
   const int64_t noted = (a.tokens ? history : 0) + a.biases;
-  a.widest = a.slice < 1 << 19 ? a.slice : 1 << 19;
   a.slots = kLogitThreads;
   while (a.slots < kSlots && a.slots * 3 / 4 < noted) a.slots *= 2;
   static_assert(kMost == kSlots * 3 / 4, "the table's size");
   static_assert(kLogitThreads * 8 <= kMost, "a block fits the table");
   switch (dtype) {
-    case MKB_F16: return launch_logits<__half>(a, M, ranks, stream);
-    case MKB_BF16: return launch_logits<__nv_bfloat16>(a, M, ranks, stream);
-    case MKB_F32: return launch_logits<float>(a, M, ranks, stream);
+    case MKB_F16: return launch_logits<__half>(a, M, stream);
+    case MKB_BF16: return launch_logits<__nv_bfloat16>(a, M, stream);
+    case MKB_F32: return launch_logits<float>(a, M, stream);
     default: break;
   }
   set_error("adjust_logits: dtype tag %d (fp16, bf16 and fp32 supported)", dtype);
