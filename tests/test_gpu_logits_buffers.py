@@ -56,13 +56,14 @@ def quickest(calls, repeats=40):
 
 @pytest.mark.parametrize("rows", [1, 8, 128])
 def test_a_short_text_in_a_wide_buffer_is_a_short_call(rows):
-    """By the width of the buffer it would take several chunks with the largest table each: 1.5 to 4 times the time."""
+    """By the width of the buffer it would take several chunks with the largest table each: 1.5 to 4 times the time.  The larger
+    table alone takes up to 1.11 times."""
     logits, tokens, arguments = given(rows, 128256, 32768, [300] * rows, torch.bfloat16)
     narrow, out = tokens[:, :300].contiguous(), torch.empty_like(logits)
     wide, fitting = quickest([lambda: kernels.adjust_logits(logits, tokens=tokens, out=out, **arguments),
                               lambda: kernels.adjust_logits(logits, tokens=narrow, out=out, **arguments)])
     print(f"{rows} rows: buffer of 32768 {wide:.1f} us, of 300 {fitting:.1f} us")
-    assert wide < 1.25 * fitting, (wide, fitting)
+    assert wide < 1.35 * fitting, (wide, fitting)
 
 
 def test_rules_at_the_length_of_a_context():

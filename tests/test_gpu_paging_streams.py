@@ -8,7 +8,7 @@ import mlkit_b200 as mk
 pytestmark = pytest.mark.gpu
 
 
-def work(seconds=0.4):
+def work(seconds=0.3):
     """Copies that keep the stream busy, and the event behind them."""
     data = torch.empty(1 << 30, dtype=torch.uint8, device="cuda"), torch.empty(1 << 30, dtype=torch.uint8, device="cuda")
     for _ in range(int(seconds * 3000)):
